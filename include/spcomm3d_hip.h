@@ -64,7 +64,15 @@ typedef enum {
     SPC3D_ERR_ALLOC = 7          /* host or device allocation failed */
 } spc3d_status;
 
-typedef enum { SPC3D_F32 = 0, SPC3D_F64 = 1 } spc3d_dtype;
+/* SDDMM, SpMM, value vectors and the row copies take the first two; panels of the others are
+ * operands of the attention calls below (F8: OCP e4m3, what a cache holds). */
+typedef enum {
+    SPC3D_F32 = 0,
+    SPC3D_F64 = 1,
+    SPC3D_BF16 = 2,
+    SPC3D_F16 = 3,
+    SPC3D_F8 = 4
+} spc3d_dtype;
 
 typedef struct spc3d_ctx spc3d_ctx;     /* device + stream */
 typedef struct spc3d_panel spc3d_panel; /* device-resident denseMatrix::data (src/basic.hpp:30-36) */
@@ -279,7 +287,8 @@ SPC3D_API int spc3d_ctx_probe_xcd(spc3d_ctx *ctx, uint32_t nblocks, uint32_t *xc
  * reference's 16384 x 16384 case runs one kernel in under 10 us).  Between
  * spc3d_capture_begin and spc3d_capture_end the calls that only queue kernels -
  * spc3d_sddmm, spc3d_spmm, spc3d_sddmm_spmm, spc3d_rows_*, spc3d_panel_fill,
- * spc3d_panel_copy, spc3d_vals_fill, spc3d_plan_set_values_device - are recorded
+ * spc3d_panel_copy, spc3d_vals_fill, spc3d_plan_set_values_device, spc3d_attend[_grad],
+ * spc3d_cache_append, spc3d_cache_attend - are recorded
  * instead of run; every other call on the context (anything that allocates,
  * copies to or from the host, waits or times) returns SPC3D_ERR_INVALID_ARG and
  * leaves the recording intact.  An SpMM over a plan with cut rows whose dense rows
@@ -543,6 +552,54 @@ SPC3D_API int spc3d_host_cache_clear(spc3d_ctx *ctx);
  * plan was reused (1) or made (0).  Any pointer may be NULL. */
 SPC3D_API int spc3d_host_call_stats(spc3d_ctx *ctx, uint64_t *bytes_sent, uint64_t *bytes_kept,
                           int *plan_reused);
+
+/* ---- attention: SDDMM, a softmax per row, SpMM, over a band ------------------
+ * The chained one-pass call with a softmax between its two products, over a pattern that needs
+ * no entries: row i of a sequence of R rows and C columns sits at position p = C - R + i and
+ * sees the columns c <= p with p - c < window (window 0: all of them) or c < sinks.  With
+ *     s_ic = scale * <q_i, k_c>,   lse_i = log sum_c exp(s_ic),   P_ic = exp(s_ic - lse_i),
+ *     o_i  = sum_c P_ic v_c        (a row that sees nothing: o_i = 0, lse_i = -inf).
+ * Nothing of the pattern or of P is ever stored.  No counterpart in the reference, which stops
+ * at the two products (src/core_ops.cpp:5-35).
+ *
+ * Operands are heads of panels: head h of token t is columns [col + h dim, col + (h+1) dim) of
+ * row t, so q, k and v may lie side by side in one panel.  Panels are SPC3D_F32, SPC3D_BF16 or
+ * SPC3D_F16, all of a call the same; sums and softmax statistics are 32-bit; the weights P and
+ * dS are rounded once to the panels' type for the second product, results once at the end.
+ * dim is a multiple of 8, at most 128; a panel's rows and `col` are whole 16-byte vectors.  The
+ * heads of q are a multiple of those of k and v: head h reads head h / (heads / kv heads).
+ *
+ * The sequences lie one after the other: rows rows[0] + .. + rows[b-1] on of q, o and their
+ * gradients are sequence b's, and likewise cols[] for k and v.  Rows and columns may be 0.
+ * scale must be positive and finite. */
+typedef struct {
+    spc3d_panel *panel;
+    uint32_t col;      /* first column */
+    uint32_t heads;
+    uint32_t dim;      /* columns of a head */
+    uint32_t reserved; /* must be 0 */
+} spc3d_heads;
+typedef struct spc3d_band spc3d_band;
+/* The pattern of a call: its sequences cut into tiles, on the device.  rows[] and cols[] (nseq
+ * each, host memory) are copied.  The first spc3d_attend_grad with a number of kv heads lays out
+ * its pieces of columns and its workspace, kept with the band (so not while recording). */
+SPC3D_API int spc3d_band_create(spc3d_ctx *ctx, uint32_t nseq, const uint32_t *rows,
+                      const uint32_t *cols, uint32_t window, uint32_t sinks, spc3d_band **out);
+SPC3D_API int spc3d_band_destroy(spc3d_band *band);
+/* lse: a value vector of floats, [row][head], or NULL.  o may not overlap q, k or v. */
+SPC3D_API int spc3d_attend(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q,
+                 const spc3d_heads *k, const spc3d_heads *v, float scale, const spc3d_heads *o,
+                 spc3d_vals *lse);
+/* The gradients of a scalar whose derivative by o is d_o, from what spc3d_attend was given and
+ * gave:  D_i = <dO_i, o_i>,  dS_ic = P_ic (<dO_i, v_c> - D_i),
+ *     dQ_i = scale sum_c dS_ic k_c,   dK_c = scale sum_i dS_ic q_i,   dV_c = sum_i P_ic dO_i,
+ * the last two over every head that shares the column's.  Overwrites dq, dk, dv (columns that no
+ * row sees get 0); runs give the same bits.  The outputs overlap neither the inputs nor each
+ * other.  Asynchronous on the context's stream, as spc3d_attend. */
+SPC3D_API int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q,
+                      const spc3d_heads *k, const spc3d_heads *v, float scale,
+                      const spc3d_heads *o, const spc3d_vals *lse, const spc3d_heads *d_o,
+                      const spc3d_heads *dq, const spc3d_heads *dk, const spc3d_heads *dv);
 
 #ifdef __cplusplus
 }

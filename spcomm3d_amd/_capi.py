@@ -15,7 +15,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "spcomm3d_hip.h")
 
 OK, ERR_INVALID_ARG, ERR_BAD_INDEX, ERR_SIZE_MISMATCH = 0, 1, 2, 3
 ERR_TOO_LARGE, ERR_NO_DEVICE, ERR_HIP, ERR_ALLOC = 4, 5, 6, 7
-F32, F64 = 0, 1
+F32, F64, BF16, F16, F8 = 0, 1, 2, 3, 4
 
 c_int, c_u32, c_u64 = ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64
 c_vp, c_double, c_float = ctypes.c_void_p, ctypes.c_double, ctypes.c_float
@@ -52,6 +52,14 @@ class PlanOpts(ctypes.Structure):
 
 PLAN_NO_STAGED_STORES, PLAN_NO_SDDMM_BY_COLUMN, PLAN_NO_TWO_PASS, PLAN_KEEP_ENTRY_ORDER = 1, 2, 4, 8
 PLAN_SWEEP_STAGED, PLAN_NO_SLICE_AFFINITY = 16, 32
+
+
+class HeadsArg(ctypes.Structure):
+    _fields_ = [("panel", c_vp), ("col", c_u32), ("heads", c_u32), ("dim", c_u32),
+                ("reserved", c_u32)]
+
+
+PH = P(HeadsArg)
 
 
 # name -> (restype, argtypes); one entry for every function the header declares.
@@ -119,6 +127,10 @@ SIGNATURES = {
                                  c_vp, c_vp]),
     "spc3d_spmm_host": (c_int, [c_vp, c_int, c_u32, c_u32, c_u32, c_vp, c_u64, c_vp, c_vp, c_vp,
                                 c_vp]),
+    "spc3d_band_create": (c_int, [c_vp, c_u32, c_vp, c_vp, c_u32, c_u32, P(c_vp)]),
+    "spc3d_band_destroy": (c_int, [c_vp]),
+    "spc3d_attend": (c_int, [c_vp, c_vp, PH, PH, PH, c_float, PH, c_vp]),
+    "spc3d_attend_grad": (c_int, [c_vp, c_vp, PH, PH, PH, c_float, PH, c_vp, PH, PH, PH, PH]),
     "spc3d_host_cache_clear": (c_int, [c_vp]),
     "spc3d_host_call_stats": (c_int, [c_vp, c_vp, c_vp, c_vp]),
 }

@@ -397,7 +397,7 @@ int spc3d_panel_create(spc3d_ctx *ctx, int dtype, uint32_t m, uint32_t n, spc3d_
     *out = nullptr;
     if (!live(ctx))
         return fail(SPC3D_ERR_INVALID_ARG, "context is NULL or destroyed");
-    if (!dtype_ok(dtype))
+    if (!panel_dtype_ok(dtype))
         return fail(SPC3D_ERR_INVALID_ARG, "unknown dtype");
     int rc = use_device(ctx);
     if (rc)
@@ -450,7 +450,7 @@ int spc3d_panel_wrap(spc3d_ctx *ctx, int dtype, uint32_t m, uint32_t n, void *de
     *out = nullptr;
     if (!live(ctx))
         return fail(SPC3D_ERR_INVALID_ARG, "context is NULL or destroyed");
-    if (!dtype_ok(dtype))
+    if (!panel_dtype_ok(dtype))
         return fail(SPC3D_ERR_INVALID_ARG, "unknown dtype");
     int rc = use_device(ctx);
     if (rc)

@@ -62,11 +62,17 @@ constexpr uint32_t kMagicVals = 0x53433356;  // instead of dereferenced further
 constexpr uint32_t kMagicPlan = 0x5343334c;
 constexpr uint32_t kMagicRowMap = 0x5343334d;
 constexpr uint32_t kMagicGraph = 0x53433347;
+constexpr uint32_t kMagicBand = 0x53433342;
 constexpr int kTimerSlots = 4096;
 constexpr uint32_t kMaxColBlocks = 4096;
 
-inline size_t elem_size(int dtype) { return dtype == SPC3D_F64 ? 8 : 4; }
+inline size_t elem_size(int dtype)
+{
+    return dtype == SPC3D_F64 ? 8 : (dtype == SPC3D_F32 ? 4 : (dtype == SPC3D_F8 ? 1 : 2));
+}
 inline bool dtype_ok(int dtype) { return dtype == SPC3D_F32 || dtype == SPC3D_F64; }
+// Panels also hold the types of the attention calls.
+inline bool panel_dtype_ok(int dtype) { return dtype >= SPC3D_F32 && dtype <= SPC3D_F8; }
 
 
 // What the one-shot entry points over host memory keep between calls: plans by the

@@ -1,0 +1,63 @@
+// Attention over a band (spc3d_attend, spc3d_attend_grad): what the host side hands to the
+// kernels of attention.hip.  Internal to the library.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace spc3d {
+
+constexpr uint32_t kKeyStep = 64;   // columns that the row kernels take at a time
+constexpr uint32_t kKeyTile = 128;  // columns of a task of the column kernel
+constexpr uint32_t kNoSlot = 0xffffffffu;
+
+// Heads of a panel: element (t, h, j) at p[t * stride + h * dim + j].
+struct HeadsView {
+    char *p;         // of the first head's first element
+    uint64_t stride; // elements from row to row
+};
+
+// A tile of rows: rows row0 .. row0 + nrow of the packed queries, at positions pos0 .. of a
+// sequence whose columns are rows key0 .. key0 + ncols of the packed keys.
+struct RowTile {
+    uint32_t row0, nrow, key0, ncols;
+    int32_t pos0;
+    uint32_t pad[3];
+};
+
+// A piece of a tile of columns: columns col0 .. col0 + nkey of their sequence, rows key0 .. of the
+// packed keys, and the rows row0 .. row0 + nrow (from position pos0 on) that this piece goes over.
+// slot: where its partial sums go, or kNoSlot for the only piece of its tile.
+struct KeyPiece {
+    uint32_t key0, nkey, row0, nrow;
+    int32_t pos0, col0;
+    uint32_t slot, pad;
+};
+
+// A tile of columns in several pieces: partial sums first .. first + count.
+struct KeySplit {
+    uint32_t key0, nkey, first, count;
+};
+
+struct BandArgs {
+    HeadsView q, k, v, o, d_o, dq, dk, dv;
+    float *lse;   // [row][head]; may be null in the forward call
+    float *delta; // [row][head], sum of d_o o
+    float *partial;
+    const RowTile *tiles;
+    const KeyPiece *pieces;
+    const KeySplit *splits;
+    uint32_t ntiles, npieces, nsplits;
+    uint32_t heads, kv_heads, dim;
+    int32_t window, sinks; // window: INT32_MAX for none
+    float scale;
+    int dtype;
+};
+
+// Rows of a tile of the forward and the dQ kernel: 64 or 128.
+hipError_t launch_attend(const BandArgs &a, uint32_t tile_rows, hipStream_t stream);
+hipError_t launch_attend_dq(const BandArgs &a, uint32_t tile_rows, hipStream_t stream);
+hipError_t launch_attend_dkv(const BandArgs &a, hipStream_t stream);
+uint64_t partial_floats(uint32_t nslots, uint32_t kv_heads, uint32_t dim);
+
+} // namespace spc3d

@@ -1,0 +1,652 @@
+// Attention over a band, forward and backward.  Row i of a sequence at position p sees column c
+// when c <= p and (p - c < window or c < sinks):
+//   s_ic = scale <q_i, k_c>,  P_ic = exp(s_ic - lse_i),  o_i = sum_c P_ic v_c
+//   dV_c = sum_i P_ic dO_i,  dS_ic = P_ic (<dO_i, v_c> - <dO_i, o_i>),
+//   dQ_i = scale sum_c dS_ic k_c,  dK_c = scale sum_i dS_ic q_i.
+#include "attention.h"
+#include "attention_frag.h"
+#include "kernels.h"
+
+namespace spc3d {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Work {
+    uint32_t tile, head;
+};
+// Workgroups go round-robin to the 8 XCDs.  With a multiple of 8 shared heads each XCD takes whole
+// shared heads, so that its L2 holds their keys and values once; otherwise in plain order, the
+// heads that share keys next to each other in time.
+__device__ __forceinline__ Work work_of(uint32_t id, uint32_t ntiles, uint32_t heads, uint32_t kv_heads)
+{
+    const uint32_t group = heads / kv_heads;
+    if (kv_heads % 8 == 0) {
+        const uint32_t j = id / 8, per = ntiles * group, r = j % per;
+        return {r / group, ((j / per) * 8 + id % 8) * group + r % group};
+    }
+    return {id / heads, id % heads};
+}
+
+// The steps of kKeyStep columns that rows at positions pa .. pb go over: `first` steps from column
+// 0 on for the sinks, then those from step `from` on.
+struct Steps {
+    int first, from, count;
+    __device__ __forceinline__ int at(int k) const { return k < first ? k : from + k - first; }
+};
+__device__ __forceinline__ Steps steps_of(int pa, int pb, int ncols, int window, int sinks)
+{
+    const int end = min(pb + 1, ncols); // columns seen lie below
+    Steps s{0, 0, 0};
+    if (end <= 0)
+        return s;
+    const int step = (int)kKeyStep;
+    const int lo = window > pa ? 0 : pa - window + 1;
+    s.first = (min(sinks, end) + step - 1) / step;
+    s.from = max(lo / step, s.first);
+    s.count = s.first + max(0, (end + step - 1) / step - s.from);
+    return s;
+}
+
+__device__ __forceinline__ bool sees(int p, int c, int window, int sinks)
+{
+    return c <= p && (p - c < window || c < sinks);
+}
+
+template <typename T> __device__ __forceinline__ bool is_finite(T x) { return fabsf((float)x) < __builtin_inff(); }
+
+// ---- forward --------------------------------------------------------------------------------
+// Each wavefront owns 16 NQ rows; K and V come through LDS in steps of 64 columns.  S^T = K Q^T
+// leaves lane l with row l % 16, so maxima and sums of a row are over the lane's own registers and
+// two exchanges, and the probabilities are the right operand of O^T += V^T P^T where they lie.
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
+{
+    typedef Tile<T, DP> L;
+    constexpr int NS = DP / 32, ND = DP / 16, NT = kKeyStep / 16;
+    __shared__ __align__(16) char smem[2 * kKeyStep * L::kRowBytes];
+    char *const kt = smem, *const vt = smem + kKeyStep * L::kRowBytes;
+
+    const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
+    const RowTile t = a.tiles[w.tile];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int dim = (int)a.dim, ncols = (int)t.ncols;
+    const uint32_t kvh = w.head / (a.heads / a.kv_heads);
+    const T *const qp = (const T *)a.q.p + t.row0 * a.q.stride + w.head * dim;
+    const T *const kp = (const T *)a.k.p + t.key0 * a.k.stride + kvh * dim;
+    const T *const vp = (const T *)a.v.p + t.key0 * a.v.stride + kvh * dim;
+
+    Frag<T> qf[NQ][NS];
+    int pos[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = (wave * NQ + n) * 16 + l;
+        pos[n] = t.pos0 + r;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int d = 32 * s + 8 * g;
+            qf[n][s] = r < (int)t.nrow && d < dim ? load_frag(qp + r * a.q.stride + d) : zero_frag<T>();
+        }
+    }
+    const Steps st = steps_of(t.pos0, t.pos0 + (int)t.nrow - 1, ncols, a.window, a.sinks);
+    const int wa = t.pos0 + wave * NQ * 16, wb = min(wa + NQ * 16, t.pos0 + (int)t.nrow) - 1;
+    const float sc = a.scale * kLog2e;
+
+    f32x4 acc[ND][NQ];
+    float m[NQ], sum[NQ];
+    TileCopy<T, DP, kKeyStep, kThreads> ck, cv;
+    // The second pass, if any, is for values that are not finite: 0 x inf would reach rows that do
+    // not see them, so steps with hidden pairs take those values one by one.
+    for (int careful = 0; careful < 2; ++careful) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            m[n] = kNegInf;
+            sum[n] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                acc[d][n] = f32x4{0, 0, 0, 0};
+        }
+        if (st.count > 0) {
+            const int c0 = st.at(0) * (int)kKeyStep;
+            ck.load(kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, tid);
+            cv.load(vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, tid);
+        }
+        for (int k = 0; k < st.count; ++k) {
+            const int c0 = st.at(k) * (int)kKeyStep;
+            __syncthreads();
+            ck.store(kt, tid);
+            cv.store(vt, tid);
+            __syncthreads();
+            if (k + 1 < st.count) {
+                const int c1 = st.at(k + 1) * (int)kKeyStep;
+                ck.load(kp + c1 * a.k.stride, a.k.stride, ncols - c1, dim, tid);
+                cv.load(vp + c1 * a.v.stride, a.v.stride, ncols - c1, dim, tid);
+            }
+            const int c9 = c0 + (int)kKeyStep - 1;
+            if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
+                continue; // nothing here is seen by this wavefront's rows
+            const bool whole = c9 <= wa && (wb - c0 < a.window || c9 < a.sinks);
+
+            f32x4 sv[NT][NQ];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+                    sv[i][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const Frag<T> f = L::rows(kt, 16 * i, s, lane);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+                        sv[i][n] = mma(f, qf[n][s], sv[i][n]);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (!sees(pos[n], c0 + 16 * i + 4 * g + j, a.window, a.sinks))
+                                sv[i][n][j] = kNegInf;
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                float top = sv[0][n][0];
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        top = fmaxf(top, sv[i][n][j]);
+                top = fmaxf(m[n], column_max(top) * sc);
+                const float base = top == kNegInf ? 0.0f : top; // nothing seen yet: exp2(-inf - 0) = 0
+                const float down = __builtin_amdgcn_exp2f(m[n] - base), less = base - WeightShift<T>::value;
+                m[n] = top;
+                float add = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i][n][j], sc, -less));
+                        sv[i][n][j] = p;
+                        add += p;
+                    }
+                sum[n] = sum[n] * down + add;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    acc[d][n] *= down;
+            }
+            const bool one_by_one = careful && !whole;
+#pragma unroll
+            for (int u = 0; u < NT / 2; ++u) {
+                Frag<T> pf[NQ];
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+                    pf[n] = join<T>(sv[2 * u][n], sv[2 * u + 1][n]);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<T> f = L::columns(vt, 32 * u, d, lane);
+                    if (one_by_one) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (!is_finite(f[j]))
+                                f[j] = (T)0.0f;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+                        acc[d][n] = mma(f, pf[n], acc[d][n]);
+                }
+            }
+            if (one_by_one) {
+                for (int c = 0; c < (int)kKeyStep; ++c)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int e = 16 * d + 4 * g + j;
+                            const T x = *reinterpret_cast<const T *>(vt + L::at(c, e / L::kVec) +
+                                                                     (e % L::kVec) * sizeof(T));
+                            if (!is_finite(x)) {
+#pragma unroll
+                                for (int n = 0; n < NQ; ++n)
+                                    if (sees(pos[n], c0 + c, a.window, a.sinks))
+                                        acc[d][n][j] += (float)x;
+                            }
+                        }
+            }
+        }
+        int bad = 0;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            sum[n] = column_sum(sum[n]);
+            const float by = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
+            const bool mine = (wave * NQ + n) * 16 + l < (int)t.nrow;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                acc[d][n] *= by;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    bad |= mine && !is_finite(acc[d][n][j]);
+            }
+        }
+        if (careful || !__syncthreads_or(bad))
+            break;
+    }
+    T *const op = (T *)a.o.p + t.row0 * a.o.stride + w.head * dim;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = (wave * NQ + n) * 16 + l;
+        if (r >= (int)t.nrow)
+            continue;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            if (16 * d + 4 * g < dim)
+                store_half<T>(op + r * a.o.stride + 16 * d + 4 * g, acc[d][n]);
+        if (a.lse && g == 0)
+            a.lse[(uint64_t)(t.row0 + r) * a.heads + w.head] =
+                sum[n] == 0.0f ? kNegInf : (m[n] + __log2f(sum[n]) - WeightShift<T>::value) * kLn2;
+    }
+}
+
+// ---- backward -------------------------------------------------------------------------------
+// Two kernels, one over rows (dQ) and one over columns (dK, dV), each with the scores computed
+// again: seven products instead of five, but every sum is one workgroup's, in a fixed order,
+// without atomics or a panel of partial dQ.
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(kThreads, 1) void attend_dq_kernel(BandArgs a)
+{
+    typedef Tile<T, DP> L;
+    constexpr int NS = DP / 32, ND = DP / 16, NT = kKeyStep / 16;
+    __shared__ __align__(16) char smem[2 * kKeyStep * L::kRowBytes];
+    char *const kt = smem, *const vt = smem + kKeyStep * L::kRowBytes;
+
+    const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
+    const RowTile t = a.tiles[w.tile];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int dim = (int)a.dim, ncols = (int)t.ncols;
+    const uint32_t kvh = w.head / (a.heads / a.kv_heads);
+    const T *const qp = (const T *)a.q.p + t.row0 * a.q.stride + w.head * dim;
+    const T *const gp = (const T *)a.d_o.p + t.row0 * a.d_o.stride + w.head * dim;
+    const T *const op = (const T *)a.o.p + t.row0 * a.o.stride + w.head * dim;
+    const T *const kp = (const T *)a.k.p + t.key0 * a.k.stride + kvh * dim;
+    const T *const vp = (const T *)a.v.p + t.key0 * a.v.stride + kvh * dim;
+
+    Frag<T> qf[NQ][NS], gf[NQ][NS];
+    int pos[NQ];
+    float lse[NQ], delta[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = (wave * NQ + n) * 16 + l;
+        const bool mine = r < (int)t.nrow;
+        pos[n] = t.pos0 + r;
+        float dot = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int d = 32 * s + 8 * g;
+            const bool in = mine && d < dim;
+            qf[n][s] = in ? load_frag(qp + r * a.q.stride + d) : zero_frag<T>();
+            gf[n][s] = in ? load_frag(gp + r * a.d_o.stride + d) : zero_frag<T>();
+            const Frag<T> of = in ? load_frag(op + r * a.o.stride + d) : zero_frag<T>();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                dot = __builtin_fmaf((float)gf[n][s][j], (float)of[j], dot);
+        }
+        delta[n] = column_sum(dot);
+        const uint64_t at = (uint64_t)(t.row0 + r) * a.heads + w.head;
+        lse[n] = mine ? a.lse[at] * kLog2e : kNegInf;
+        if (lse[n] == kNegInf)
+            lse[n] = -kNegInf; // a row that sees nothing: every weight is exp2(-inf)
+        if (mine && g == 0)
+            a.delta[at] = delta[n];
+    }
+    const Steps st = steps_of(t.pos0, t.pos0 + (int)t.nrow - 1, ncols, a.window, a.sinks);
+    const int wa = t.pos0 + wave * NQ * 16, wb = min(wa + NQ * 16, t.pos0 + (int)t.nrow) - 1;
+    const float sc = a.scale * kLog2e;
+
+    f32x4 acc[ND][NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            acc[d][n] = f32x4{0, 0, 0, 0};
+    TileCopy<T, DP, kKeyStep, kThreads> ck, cv;
+    if (st.count > 0) {
+        const int c0 = st.at(0) * (int)kKeyStep;
+        ck.load(kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, tid);
+        cv.load(vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, tid);
+    }
+    for (int k = 0; k < st.count; ++k) {
+        const int c0 = st.at(k) * (int)kKeyStep;
+        __syncthreads();
+        ck.store(kt, tid);
+        cv.store(vt, tid);
+        __syncthreads();
+        if (k + 1 < st.count) {
+            const int c1 = st.at(k + 1) * (int)kKeyStep;
+            ck.load(kp + c1 * a.k.stride, a.k.stride, ncols - c1, dim, tid);
+            cv.load(vp + c1 * a.v.stride, a.v.stride, ncols - c1, dim, tid);
+        }
+        const int c9 = c0 + (int)kKeyStep - 1;
+        if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
+            continue;
+        const bool whole = c9 <= wa && (wb - c0 < a.window || c9 < a.sinks);
+#pragma unroll
+        for (int u = 0; u < NT / 2; ++u) {
+            f32x4 sv[2][NQ], dp[2][NQ];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+                    sv[i][n] = dp[i][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const Frag<T> f = L::rows(kt, 32 * u + 16 * i, s, lane);
+                    const Frag<T> h = L::rows(vt, 32 * u + 16 * i, s, lane);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        sv[i][n] = mma(f, qf[n][s], sv[i][n]);
+                        dp[i][n] = mma(h, gf[n][s], dp[i][n]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i][n][j], sc, -lse[n]));
+                        float ds = p * (dp[i][n][j] - delta[n]);
+                        if (!whole && !sees(pos[n], c0 + 32 * u + 16 * i + 4 * g + j, a.window, a.sinks))
+                            ds = 0.0f;
+                        sv[i][n][j] = ds;
+                    }
+            }
+            Frag<T> df[NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+                df[n] = join<T>(sv[0][n], sv[1][n]);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const Frag<T> f = L::columns(kt, 32 * u, d, lane);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+                    acc[d][n] = mma(f, df[n], acc[d][n]);
+            }
+        }
+    }
+    T *const dqp = (T *)a.dq.p + t.row0 * a.dq.stride + w.head * dim;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = (wave * NQ + n) * 16 + l;
+        if (r >= (int)t.nrow)
+            continue;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            if (16 * d + 4 * g < dim)
+                store_half<T>(dqp + r * a.dq.stride + 16 * d + 4 * g, acc[d][n] * a.scale);
+    }
+}
+
+// Each wavefront owns 32 columns of the tile's 128, whose keys and values stay in its registers;
+// rows (of every head that shares them) come through LDS 32 at a time.  S = Q K^T leaves a lane
+// with one column and the rows 4 g + i, 16 + 4 g + i, which is the left operand of dV += P^T dO and
+// dK += dS^T Q as it lies.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 1) void attend_dkv_kernel(BandArgs a)
+{
+    typedef Tile<T, DP> L;
+    constexpr int NS = DP / 32, ND = DP / 16, NK = 2, ROWS = 32;
+    constexpr float kUp = WeightShift<T>::value ? 32768.0f : 1.0f;
+    __shared__ __align__(16) char smem[2 * ROWS * L::kRowBytes];
+    __shared__ __align__(16) float row_lse[ROWS], row_delta[ROWS];
+    char *const qt = smem, *const gt = smem + ROWS * L::kRowBytes;
+
+    const uint32_t group = a.heads / a.kv_heads;
+    const Work w = work_of(blockIdx.x, a.npieces, a.kv_heads, a.kv_heads);
+    const KeyPiece t = a.pieces[w.tile];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int dim = (int)a.dim, nrow = (int)t.nrow;
+    const T *const kp = (const T *)a.k.p + t.key0 * a.k.stride + w.head * dim;
+    const T *const vp = (const T *)a.v.p + t.key0 * a.v.stride + w.head * dim;
+
+    Frag<T> kf[NK][NS], vf[NK][NS];
+    f32x4 dk[NK][ND], dv[NK][ND];
+    int col[NK];
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+        const int r = (wave * NK + n) * 16 + l;
+        col[n] = t.col0 + r;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int d = 32 * s + 8 * g;
+            const bool in = r < (int)t.nkey && d < dim;
+            kf[n][s] = in ? load_frag(kp + r * a.k.stride + d) : zero_frag<T>();
+            vf[n][s] = in ? load_frag(vp + r * a.v.stride + d) : zero_frag<T>();
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            dk[n][d] = dv[n][d] = f32x4{0, 0, 0, 0};
+    }
+    const int ca = t.col0 + wave * NK * 16, cb = ca + NK * 16 - 1;
+    const float sc = a.scale * kLog2e;
+    const int per = (nrow + ROWS - 1) / ROWS, count = per * (int)group;
+
+    TileCopy<T, DP, ROWS, kThreads> cq, cg;
+    float next_lse = 0.0f, next_delta = 0.0f;
+    auto fetch = [&](int k) {
+        const uint32_t head = w.head * group + k / per;
+        const int r0 = (k % per) * ROWS;
+        const uint64_t row = t.row0 + r0;
+        cq.load((const T *)a.q.p + row * a.q.stride + head * dim, a.q.stride, nrow - r0, dim, tid);
+        cg.load((const T *)a.d_o.p + row * a.d_o.stride + head * dim, a.d_o.stride, nrow - r0, dim, tid);
+        if (tid < ROWS) {
+            next_lse = -kNegInf; // rows past the end and rows that see nothing weigh nothing
+            next_delta = 0.0f;
+            if (r0 + tid < nrow) {
+                const float x = a.lse[(row + tid) * a.heads + head] * kLog2e;
+                next_lse = x == kNegInf ? -kNegInf : x;
+                next_delta = a.delta[(row + tid) * a.heads + head];
+            }
+        }
+    };
+    if (count > 0)
+        fetch(0);
+    for (int k = 0; k < count; ++k) {
+        __syncthreads();
+        cq.store(qt, tid);
+        cg.store(gt, tid);
+        if (tid < ROWS) {
+            row_lse[tid] = next_lse;
+            row_delta[tid] = next_delta;
+        }
+        __syncthreads();
+        if (k + 1 < count)
+            fetch(k + 1);
+        const int pa = t.pos0 + (k % per) * ROWS, pb = pa + ROWS - 1;
+        if (pb < ca || (pa - cb >= a.window && ca >= a.sinks))
+            continue;
+        const bool whole = pa >= cb && (pb - ca < a.window || cb < a.sinks);
+
+        f32x4 sv[2][NK], dp[2][NK];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+                sv[i][n] = dp[i][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const Frag<T> f = L::rows(qt, 16 * i, s, lane);
+                const Frag<T> h = L::rows(gt, 16 * i, s, lane);
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    sv[i][n] = mma(f, kf[n][s], sv[i][n]);
+                    dp[i][n] = mma(h, vf[n][s], dp[i][n]);
+                }
+            }
+            const f32x4 lse = *reinterpret_cast<const f32x4 *>(row_lse + 16 * i + 4 * g);
+            const f32x4 delta = *reinterpret_cast<const f32x4 *>(row_delta + 16 * i + 4 * g);
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i][n][j], sc, -lse[j]));
+                    float ds = p * (dp[i][n][j] - delta[j]);
+                    p *= kUp;
+                    if (!whole && !sees(pa + 16 * i + 4 * g + j, col[n], a.window, a.sinks))
+                        p = ds = 0.0f;
+                    sv[i][n][j] = p;
+                    dp[i][n][j] = ds;
+                }
+        }
+        Frag<T> pf[NK], df[NK];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+            pf[n] = join<T>(sv[0][n], sv[1][n]);
+            df[n] = join<T>(dp[0][n], dp[1][n]);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const Frag<T> f = L::columns(gt, 0, d, lane);
+            const Frag<T> h = L::columns(qt, 0, d, lane);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                dv[n][d] = mma(pf[n], f, dv[n][d]);
+                dk[n][d] = mma(df[n], h, dk[n][d]);
+            }
+        }
+    }
+    // lane l holds element 16 d + l of the columns 4 g + j
+    T *const dkp = (T *)a.dk.p + t.key0 * a.dk.stride + w.head * dim;
+    T *const dvp = (T *)a.dv.p + t.key0 * a.dv.stride + w.head * dim;
+    float *const part = t.slot == kNoSlot
+                            ? nullptr
+                            : a.partial + ((uint64_t)t.slot * a.kv_heads + w.head) * 2 * kKeyTile * dim;
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = (wave * NK + n) * 16 + 4 * g + j;
+            if (c >= (int)t.nkey)
+                continue;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const int e = 16 * d + l;
+                if (e >= dim)
+                    continue;
+                if (part) {
+                    part[c * dim + e] = dk[n][d][j];
+                    part[(kKeyTile + c) * dim + e] = dv[n][d][j] * (1.0f / kUp);
+                } else {
+                    dkp[c * a.dk.stride + e] = (T)(dk[n][d][j] * a.scale);
+                    dvp[c * a.dv.stride + e] = (T)(dv[n][d][j] * (1.0f / kUp));
+                }
+            }
+        }
+}
+
+// The pieces of a tile of columns joined in their order.
+template <typename T> __global__ __launch_bounds__(kThreads) void join_dkv_kernel(BandArgs a)
+{
+    const KeySplit t = a.splits[blockIdx.x];
+    const uint32_t h = blockIdx.y, dim = a.dim;
+    const uint64_t step = (uint64_t)a.kv_heads * 2 * kKeyTile * dim;
+    const float *const part = a.partial + ((uint64_t)t.first * a.kv_heads + h) * 2 * kKeyTile * dim;
+    for (uint32_t i = blockIdx.z * kThreads + threadIdx.x; i < t.nkey * dim; i += gridDim.z * kThreads) {
+        const uint32_t c = i / dim, e = i % dim;
+        float x = 0.0f, y = 0.0f;
+        for (uint32_t s = 0; s < t.count; ++s) {
+            x += part[s * step + i];
+            y += part[s * step + kKeyTile * dim + i];
+        }
+        ((T *)a.dk.p)[(t.key0 + c) * a.dk.stride + h * dim + e] = (T)(x * a.scale);
+        ((T *)a.dv.p)[(t.key0 + c) * a.dv.stride + h * dim + e] = (T)y;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void fill_short_kernel(int dtype, void *p, uint64_t n, float value)
+{
+    const bf16_t b = (bf16_t)value;
+    const f16_t h = (f16_t)value;
+    const uint16_t w = dtype == 2 ? __builtin_bit_cast(uint16_t, b) : __builtin_bit_cast(uint16_t, h);
+    for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (uint64_t)gridDim.x * kThreads)
+        if (dtype == 4)
+            ((uint8_t *)p)[i] = to_f8(value);
+        else
+            ((uint16_t *)p)[i] = w;
+}
+
+enum class Op { kForward, kDq, kDkv };
+
+template <typename T, int DP> void launch_one(const BandArgs &a, Op op, uint32_t tile_rows, hipStream_t s)
+{
+    const dim3 block(kThreads), rows(a.ntiles * a.heads);
+    if (op == Op::kDkv)
+        hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(a.npieces * a.kv_heads), block, 0, s, a);
+    else if (op == Op::kDq && tile_rows == 128)
+        hipLaunchKernelGGL((attend_dq_kernel<T, DP, 2>), rows, block, 0, s, a);
+    else if (op == Op::kDq)
+        hipLaunchKernelGGL((attend_dq_kernel<T, DP, 1>), rows, block, 0, s, a);
+    else if (tile_rows == 128)
+        hipLaunchKernelGGL((attend_kernel<T, DP, 2>), rows, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((attend_kernel<T, DP, 1>), rows, block, 0, s, a);
+}
+
+// Heads are computed as if they had 64, 96 or 128 elements (32 bits: 64 or 128), zeros behind their own.
+hipError_t launch(const BandArgs &a, Op op, uint32_t tile_rows, hipStream_t s)
+{
+    const int dp = a.dim <= 64 ? 64 : (a.dim <= 96 && a.dtype != 0 ? 96 : 128);
+    switch (a.dtype * 1000 + dp) {
+    case 64: launch_one<float, 64>(a, op, tile_rows, s); break;
+    case 128: launch_one<float, 128>(a, op, tile_rows, s); break;
+    case 2064: launch_one<bf16_t, 64>(a, op, tile_rows, s); break;
+    case 2096: launch_one<bf16_t, 96>(a, op, tile_rows, s); break;
+    case 2128: launch_one<bf16_t, 128>(a, op, tile_rows, s); break;
+    case 3064: launch_one<f16_t, 64>(a, op, tile_rows, s); break;
+    case 3096: launch_one<f16_t, 96>(a, op, tile_rows, s); break;
+    case 3128: launch_one<f16_t, 128>(a, op, tile_rows, s); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+} // namespace
+
+hipError_t launch_attend(const BandArgs &a, uint32_t tile_rows, hipStream_t stream)
+{
+    return a.ntiles ? launch(a, Op::kForward, tile_rows, stream) : hipSuccess;
+}
+
+hipError_t launch_attend_dq(const BandArgs &a, uint32_t tile_rows, hipStream_t stream)
+{
+    return a.ntiles ? launch(a, Op::kDq, tile_rows, stream) : hipSuccess;
+}
+
+hipError_t launch_attend_dkv(const BandArgs &a, hipStream_t stream)
+{
+    if (!a.npieces)
+        return hipSuccess;
+    hipError_t e = launch(a, Op::kDkv, 0, stream);
+    if (e != hipSuccess || !a.nsplits)
+        return e;
+    const dim3 grid(a.nsplits, a.kv_heads, (kKeyTile * a.dim + 4 * kThreads - 1) / (4 * kThreads));
+    switch (a.dtype) {
+    case 0: hipLaunchKernelGGL((join_dkv_kernel<float>), grid, dim3(kThreads), 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((join_dkv_kernel<bf16_t>), grid, dim3(kThreads), 0, stream, a); break;
+    default: hipLaunchKernelGGL((join_dkv_kernel<f16_t>), grid, dim3(kThreads), 0, stream, a); break;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_fill_short(int dtype, void *p, uint64_t n, float value, hipStream_t stream)
+{
+    const uint32_t grid = (uint32_t)((n + kThreads - 1) / kThreads < 4096 ? (n + kThreads - 1) / kThreads : 4096);
+    hipLaunchKernelGGL(fill_short_kernel, dim3(grid), dim3(kThreads), 0, stream, dtype, p, n, value);
+    return hipGetLastError();
+}
+
+uint64_t partial_floats(uint32_t nslots, uint32_t kv_heads, uint32_t dim)
+{
+    return (uint64_t)nslots * kv_heads * 2 * kKeyTile * dim;
+}
+
+} // namespace spc3d

@@ -13,6 +13,12 @@ _DT = {np.dtype(np.float32): capi.F32, np.dtype(np.float64): capi.F64}
 _NP = {capi.F32: np.dtype(np.float32), capi.F64: np.dtype(np.float64)}
 
 
+# Types of panels beside those of SDDMM and SpMM, by name; bfloat16 and e4m3 have no numpy type
+# and are uploaded and downloaded as their bits.
+_SHORT = {"bf16": (capi.BF16, np.dtype(np.uint16)), "f16": (capi.F16, np.dtype(np.float16)),
+          "f8": (capi.F8, np.dtype(np.uint8))}
+
+
 def dtype_code(dtype) -> int:
     if isinstance(dtype, str):
         dtype = {"f32": np.float32, "f64": np.float64}.get(dtype, dtype)
@@ -118,8 +124,8 @@ class Context:
         return float(ms.value)
 
     # -- factories ---------------------------------------------------------
-    def panel(self, m: int, n: int, dtype) -> "Panel":
-        return Panel(self, m, n, dtype)
+    def panel(self, m: int, n: int, dtype, dev: int | None = None) -> "Panel":
+        return Panel(self, m, n, dtype, dev)
 
     def panel_from(self, host: np.ndarray) -> "Panel":
         host = np.ascontiguousarray(host)
@@ -176,6 +182,32 @@ class Context:
         cut rows live in an array that is part of the library's device code."""
         check(self._lib.spc3d_spmm_noalloc(self._h, A._h, X._h, Y._h), "spc3d_spmm_noalloc")
 
+    # -- attention ---------------------------------------------------------
+    def band(self, rows, cols=None, window: int = 0, sinks: int = 0) -> "Band":
+        """Sequences of ``rows[b]`` queries over ``cols[b]`` keys (default: as many), each row
+        seeing the last ``window`` columns up to its own (0: all) and the first ``sinks``."""
+        return Band(self, rows, cols, window, sinks)
+
+    def attend(self, band: "Band", q: "Heads", k: "Heads", v: "Heads", o: "Heads",
+               lse: "Vals | None" = None, scale: float | None = None):
+        """o = softmax(scale q k^T) v over the band (``spc3d_attend``); ``scale``: 1 / sqrt(dim)
+        unless given; asynchronous."""
+        rc = self._lib.spc3d_attend(self._h, band._h, q._ref, k._ref, v._ref,
+                                    q.dim ** -0.5 if scale is None else scale, o._ref,
+                                    None if lse is None else lse._h)
+        if rc:
+            check(rc, "spc3d_attend")
+
+    def attend_grad(self, band: "Band", q: "Heads", k: "Heads", v: "Heads", o: "Heads", lse: "Vals",
+                    d_o: "Heads", dq: "Heads", dk: "Heads", dv: "Heads", scale: float | None = None):
+        """Gradients by q, k and v from the derivative ``d_o`` by o (``spc3d_attend_grad``);
+        asynchronous."""
+        rc = self._lib.spc3d_attend_grad(self._h, band._h, q._ref, k._ref, v._ref,
+                                         q.dim ** -0.5 if scale is None else scale, o._ref, lse._h,
+                                         d_o._ref, dq._ref, dk._ref, dv._ref)
+        if rc:
+            check(rc, "spc3d_attend_grad")
+
     def sddmm_host(self, A: np.ndarray, B: np.ndarray, ii, jj, svv: np.ndarray) -> np.ndarray:
         """One-shot SDDMM over host arrays (``spc3d_sddmm_host``); returns C.vv."""
         A, B, svv = (np.ascontiguousarray(x) for x in (A, B, svv))
@@ -217,8 +249,11 @@ class Panel:
     def __init__(self, ctx: Context, m: int, n: int, dtype, dev: int | None = None):
         """``dev``: a device address to wrap (``spc3d_panel_wrap``) instead of allocating."""
         self.ctx, self.m, self.n = ctx, int(m), int(n)
-        self.code = dtype_code(dtype)
-        self.dtype = _NP[self.code]
+        if isinstance(dtype, str) and dtype in _SHORT:
+            self.code, self.dtype = _SHORT[dtype]
+        else:
+            self.code = dtype_code(dtype)
+            self.dtype = _NP[self.code]
         h = ctypes.c_void_p()
         if dev is None:
             check(ctx._lib.spc3d_panel_create(ctx._h, self.code, self.m, self.n, ctypes.byref(h)),
@@ -243,6 +278,10 @@ class Panel:
     def fill(self, value: float):
         check(self.ctx._lib.spc3d_panel_fill(self._h, float(value)), "spc3d_panel_fill")
 
+    def heads(self, heads: int, dim: int, col: int = 0) -> "Heads":
+        """Columns ``col`` on as ``heads`` heads of ``dim`` columns (``spc3d_heads``)."""
+        return Heads(self, heads, dim, col)
+
     def copy_from(self, src: "Panel"):
         """self = src on the device (``spc3d_panel_copy``); asynchronous."""
         check(self.ctx._lib.spc3d_panel_copy(self._h, src._h), "spc3d_panel_copy")
@@ -256,6 +295,42 @@ class Panel:
     def close(self):
         if getattr(self, "_h", None) and getattr(self.ctx, "_h", None):
             self.ctx._lib.spc3d_panel_destroy(self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Heads:
+    """Heads of a panel, the operand of the attention calls (``spc3d_heads``)."""
+
+    def __init__(self, panel: Panel, heads: int, dim: int, col: int = 0):
+        self.panel, self.nheads, self.dim, self.col = panel, int(heads), int(dim), int(col)
+        self._arg = capi.HeadsArg(panel._h, self.col, self.nheads, self.dim, 0)
+        self._ref = ctypes.byref(self._arg)
+
+
+class Band:
+    """The pattern of attention over a window and the first columns, for sequences that lie one
+    after the other (``spc3d_band``)."""
+
+    def __init__(self, ctx: Context, rows, cols=None, window: int = 0, sinks: int = 0):
+        rows = _as_idx(rows, "rows")
+        cols = rows if cols is None else _as_idx(cols, "cols")
+        if rows.shape != cols.shape or rows.ndim != 1:
+            raise ValueError("rows and cols must be 1-D arrays of the same length")
+        self.ctx = ctx
+        h = ctypes.c_void_p()
+        check(ctx._lib.spc3d_band_create(ctx._h, rows.size, _vp(rows), _vp(cols), int(window),
+                                         int(sinks), ctypes.byref(h)), "spc3d_band_create")
+        self._h = h
+
+    def close(self):
+        if getattr(self, "_h", None) and getattr(self.ctx, "_h", None):
+            self.ctx._lib.spc3d_band_destroy(self._h)
         self._h = None
 
     def __del__(self):
