@@ -601,6 +601,67 @@ SPC3D_API int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_he
                       const spc3d_heads *o, const spc3d_vals *lse, const spc3d_heads *d_o,
                       const spc3d_heads *dq, const spc3d_heads *dk, const spc3d_heads *dv);
 
+/* ---- a paged cache of keys and values ---------------------------------------
+ * For sequences that grow token by token: the rows of k and v that attention goes back to, kept
+ * in pages of `page` tokens (16, 32, 64 or 128) that belong to sequences by a table, as the rows
+ * of a panel belong to buffer slots by a row map.  A page holds, for every head,
+ *     keys   [page id][head][slot][dim],   values [page id][head][dim][slot]
+ * (values by element, which is how the product with the weights reads them), in SPC3D_BF16,
+ * SPC3D_F16 or SPC3D_F8; in 8 bits beside either a float for each page and head, [page id][head],
+ * and a code stands for code * scale.  dim: a multiple of 8 (8 bits: of 16), at most 128.
+ * spc3d_cache_wrap takes the caller's own device memory for it, as spc3d_panel_wrap does
+ * (k_scale, v_scale: NULL unless in 8 bits). */
+typedef struct spc3d_cache spc3d_cache;
+SPC3D_API int spc3d_cache_create(spc3d_ctx *ctx, int dtype, uint32_t npages, uint32_t page,
+                       uint32_t heads, uint32_t dim, spc3d_cache **out);
+SPC3D_API int spc3d_cache_wrap(spc3d_ctx *ctx, int dtype, uint32_t npages, uint32_t page,
+                     uint32_t heads, uint32_t dim, void *k, void *v, void *k_scale, void *v_scale,
+                     spc3d_cache **out);
+SPC3D_API int spc3d_cache_destroy(spc3d_cache *cache);
+/* Where it lies on the device; any pointer may be NULL.  Scales are NULL unless in 8 bits. */
+SPC3D_API int spc3d_cache_device_ptrs(spc3d_cache *cache, void **k, void **v, void **k_scale,
+                            void **v_scale);
+/* The sequences of a call, in device memory (4-byte aligned, of the context's GPU), read when the
+ * call runs: a recorded call sees what they hold at launch.  Rows starts[b] .. starts[b+1] of the
+ * panels are the newest tokens of sequence b (starts ascend and end at `rows`); it holds lens[b]
+ * tokens with them, token t in slot t % page of page table[b * table_stride + t / page].  The
+ * bounds are what the launches are sized for: rows and tokens past them are left alone, as are
+ * tokens in pages of a number the cache does not have (no row sees them). */
+typedef struct {
+    uint32_t nseq;
+    uint32_t table_stride; /* entries of the table for each sequence */
+    uint32_t rows;         /* of all sequences */
+    uint32_t max_rows;     /* of a sequence, at most */
+    uint32_t max_len;      /* tokens of a sequence, at most */
+    uint32_t reserved;     /* must be 0 */
+    const void *table;     /* uint32 [nseq * table_stride] */
+    const void *lens;      /* uint32 [nseq] */
+    const void *starts;    /* uint32 [nseq + 1] */
+} spc3d_cache_seqs;
+/* The rows of k and v go to the cache (panels: SPC3D_BF16 or SPC3D_F16, the cache's own type
+ * unless that is 8 bits).  rotations, unless NULL, is a panel of floats with a row for every
+ * position below max_len: cosines, then sines of n / 2 angles (n a multiple of 16, at most dim).
+ * The keys, and the rows of q on their way to q_out (unless both are NULL), are rotated by it: elements
+ * x_j and x_{j+n/2} of a head become x_j cos_j - x_{j+n/2} sin_j and x_{j+n/2} cos_j + x_j sin_j,
+ * in 32 bits, those from n on stay.
+ * In 8 bits the scale of a page and head is the smallest power of two 2^e, -40 <= e <= 40, that
+ * brings the largest finite of its values to at most 448, and never below the one it has, unless the call
+ * writes the page's first slot; what the page holds is rounded again when it grows.  Values beyond
+ * 448 scales become that, NaN stays.  A page of one sequence only may be appended to.
+ * Asynchronous on the context's stream; may be recorded. */
+SPC3D_API int spc3d_cache_append(spc3d_ctx *ctx, spc3d_cache *cache, const spc3d_cache_seqs *seqs,
+                       const spc3d_heads *k, const spc3d_heads *v, const spc3d_panel *rotations,
+                       const spc3d_heads *q, const spc3d_heads *q_out);
+/* o = softmax(scale q K^T) V of every row over its sequence's cached tokens, as spc3d_attend over a
+ * band: row i of n sits at position lens - n + i and sees the tokens t at or before it with
+ * position - t < window (0: all) or t < sinks.  Pages between the first `sinks` tokens and the
+ * window are not read: their table entries may name anything.  lse as there.  With few rows the
+ * tokens of a sequence are shared out to several workgroups; their sums lie in a workspace of the
+ * cache, which grows on first use (so not while recording).  Asynchronous on the context's stream. */
+SPC3D_API int spc3d_cache_attend(spc3d_ctx *ctx, spc3d_cache *cache, const spc3d_cache_seqs *seqs,
+                       const spc3d_heads *q, float scale, uint32_t window, uint32_t sinks,
+                       const spc3d_heads *o, spc3d_vals *lse);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,15 @@ class HeadsArg(ctypes.Structure):
 PH = P(HeadsArg)
 
 
+class CacheSeqsArg(ctypes.Structure):
+    _fields_ = [("nseq", c_u32), ("table_stride", c_u32), ("rows", c_u32), ("max_rows", c_u32),
+                ("max_len", c_u32), ("reserved", c_u32), ("table", c_vp), ("lens", c_vp),
+                ("starts", c_vp)]
+
+
+PS = P(CacheSeqsArg)
+
+
 # name -> (restype, argtypes); one entry for every function the header declares.
 SIGNATURES = {
     "spc3d_version": (ctypes.c_char_p, []),
@@ -131,6 +140,13 @@ SIGNATURES = {
     "spc3d_band_destroy": (c_int, [c_vp]),
     "spc3d_attend": (c_int, [c_vp, c_vp, PH, PH, PH, c_float, PH, c_vp]),
     "spc3d_attend_grad": (c_int, [c_vp, c_vp, PH, PH, PH, c_float, PH, c_vp, PH, PH, PH, PH]),
+    "spc3d_cache_create": (c_int, [c_vp, c_int, c_u32, c_u32, c_u32, c_u32, P(c_vp)]),
+    "spc3d_cache_wrap": (c_int, [c_vp, c_int, c_u32, c_u32, c_u32, c_u32, c_vp, c_vp, c_vp, c_vp,
+                                 P(c_vp)]),
+    "spc3d_cache_destroy": (c_int, [c_vp]),
+    "spc3d_cache_device_ptrs": (c_int, [c_vp, P(c_vp), P(c_vp), P(c_vp), P(c_vp)]),
+    "spc3d_cache_append": (c_int, [c_vp, c_vp, PS, PH, PH, c_vp, PH, PH]),
+    "spc3d_cache_attend": (c_int, [c_vp, c_vp, PS, PH, c_float, c_u32, c_u32, PH, c_vp]),
     "spc3d_host_cache_clear": (c_int, [c_vp]),
     "spc3d_host_call_stats": (c_int, [c_vp, c_vp, c_vp, c_vp]),
 }

@@ -419,29 +419,6 @@ int spc3d_panel_create(spc3d_ctx *ctx, int dtype, uint32_t m, uint32_t n, spc3d_
     return SPC3D_OK;
 }
 
-namespace {
-// `dev` must be `bytes` of device memory of ctx's GPU, 16-byte aligned (the copy and
-// pack kernels move 16-byte vectors from the start of a buffer).
-int check_wrapped(spc3d_ctx *ctx, const void *dev, size_t bytes)
-{
-    if (bytes == 0)
-        return SPC3D_OK;
-    if (!dev)
-        return fail(SPC3D_ERR_INVALID_ARG, "device pointer is NULL");
-    if (reinterpret_cast<uintptr_t>(dev) % 16)
-        return fail(SPC3D_ERR_INVALID_ARG, "device pointer is not 16-byte aligned");
-    hipPointerAttribute_t at;
-    std::memset(&at, 0, sizeof at);
-    if (hipPointerGetAttributes(&at, dev) != hipSuccess) {
-        (void)hipGetLastError();
-        return fail(SPC3D_ERR_INVALID_ARG, "pointer is not known to the HIP runtime");
-    }
-    if (at.type != hipMemoryTypeDevice || at.device != ctx->device)
-        return fail(SPC3D_ERR_INVALID_ARG, "pointer is not device memory of the context's GPU");
-    return SPC3D_OK;
-}
-} // namespace
-
 int spc3d_panel_wrap(spc3d_ctx *ctx, int dtype, uint32_t m, uint32_t n, void *dev,
                      spc3d_panel **out)
 {

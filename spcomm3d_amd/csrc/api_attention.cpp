@@ -2,6 +2,7 @@
 // workspace, the launches of attention.hip.
 #include "api_internal.h"
 #include "attention.h"
+#include "cache.h"
 
 #include <algorithm>
 #include <climits>
@@ -35,8 +36,19 @@ struct spc3d_band {
     std::vector<void *> retired;
 };
 
+struct spc3d_cache {
+    uint32_t magic;
+    spc3d_ctx *ctx;
+    CacheView view;
+    bool owned = true; // false: the caller's device memory (spc3d_cache_wrap)
+    float *work = nullptr; // sums of the workgroups that share a sequence, see spc3d_band
+    uint64_t work_floats = 0;
+    std::vector<void *> retired;
+};
+
 namespace {
 
+inline bool live(const spc3d_cache *c) { return c && c->magic == kMagicCache && live(c->ctx); }
 inline bool live(const spc3d_band *b) { return b && b->magic == kMagicBand && live(b->ctx); }
 
 void free_band(spc3d_band *b)
@@ -187,7 +199,8 @@ int schedule_of(spc3d_band *b, uint32_t kv_heads, KeySchedule **out)
     return SPC3D_OK;
 }
 
-int ensure_work(spc3d_band *b, uint64_t floats)
+// The workspace of a band or a cache with room for so many floats.
+template <typename H> int ensure_work(H *b, uint64_t floats)
 {
     if (floats <= b->work_floats)
         return SPC3D_OK;
@@ -466,6 +479,288 @@ int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q, co
     a.nsplits = s->nsplits;
     HIP_TRY(launch_attend_dq(a, tile_rows, ctx->stream));
     HIP_TRY(launch_attend_dkv(a, ctx->stream));
+    return SPC3D_OK;
+}
+
+/* ---- the paged cache ------------------------------------------------------ */
+
+namespace {
+
+int make_cache(spc3d_ctx *ctx, int dtype, uint32_t npages, uint32_t page, uint32_t heads, uint32_t dim,
+               void *const *mem, spc3d_cache **out)
+{
+    if (!out)
+        return fail(SPC3D_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    if (!live(ctx))
+        return fail(SPC3D_ERR_INVALID_ARG, "context is NULL or destroyed");
+    if (dtype != SPC3D_BF16 && dtype != SPC3D_F16 && dtype != SPC3D_F8)
+        return fail(SPC3D_ERR_INVALID_ARG, "a cache holds bfloat16, half or 8 bits");
+    if (page != 16 && page != 32 && page != 64 && page != 128)
+        return fail(SPC3D_ERR_INVALID_ARG, "pages have 16, 32, 64 or 128 tokens");
+    if (!heads || !dim || dim > 128 || dim % (dtype == SPC3D_F8 ? 16 : 8))
+        return fail(SPC3D_ERR_INVALID_ARG, "a cache needs heads of 8, 16, .. 128 elements (8 bits: 16, 32, ..)");
+    if (heads > 65535 || npages == UINT32_MAX)
+        return fail(SPC3D_ERR_TOO_LARGE, "more than 65535 heads or 2^32 - 2 pages");
+    int rc = use_device(ctx);
+    if (rc)
+        return rc;
+    const uint64_t units = (uint64_t)npages * heads;
+    const bool f8 = dtype == SPC3D_F8;
+    const size_t bytes[4] = {(size_t)units * page * dim * elem_size(dtype), (size_t)units * page * dim * elem_size(dtype),
+                             f8 ? (size_t)units * 4 : 0, f8 ? (size_t)units * 4 : 0};
+    void *at[4] = {nullptr, nullptr, nullptr, nullptr};
+    if (mem) {
+        for (int i = 0; i < 4 && !rc; ++i) {
+            if (i >= 2 && !f8 && mem[i])
+                return fail(SPC3D_ERR_INVALID_ARG, "scales belong to a cache in 8 bits");
+            rc = check_wrapped(ctx, mem[i], bytes[i]);
+            for (int j = 0; j < i && !rc; ++j)
+                if (bytes[i] && ranges_overlap(mem[i], bytes[i], mem[j], bytes[j]))
+                    rc = fail(SPC3D_ERR_INVALID_ARG, "keys, values and scales overlap");
+            at[i] = bytes[i] ? mem[i] : nullptr;
+        }
+        if (rc)
+            return rc;
+    }
+    spc3d_cache *c = new (std::nothrow) spc3d_cache();
+    if (!c)
+        return fail(SPC3D_ERR_ALLOC, "host allocation failed");
+    c->ctx = ctx;
+    c->owned = !mem;
+    for (int i = 0; i < 4 && !mem && !rc; ++i)
+        rc = dev_alloc_bytes(ctx, &at[i], bytes[i]);
+    if (rc) {
+        for (void *p : at)
+            if (p) (void)hipFree(p);
+        delete c;
+        return rc;
+    }
+    c->view = CacheView{(char *)at[0], (char *)at[1], (float *)at[2], (float *)at[3], npages, page, heads, dim, dtype};
+    c->magic = kMagicCache;
+    *out = c;
+    return SPC3D_OK;
+}
+
+int check_seqs(const spc3d_cache_seqs *s)
+{
+    if (!s)
+        return fail(SPC3D_ERR_INVALID_ARG, "seqs is NULL");
+    if (s->reserved)
+        return fail(SPC3D_ERR_INVALID_ARG, "reserved word of spc3d_cache_seqs set");
+    if (s->nseq && s->rows && (!s->table || !s->lens || !s->starts))
+        return fail(SPC3D_ERR_INVALID_ARG, "table, lens or starts is NULL");
+    for (const void *p : {s->table, s->lens, s->starts})
+        if (reinterpret_cast<uintptr_t>(p) % 4)
+            return fail(SPC3D_ERR_INVALID_ARG, "table, lens or starts is not 4-byte aligned");
+    if (s->max_len > (uint32_t)INT_MAX / 2 || s->max_rows > (uint32_t)INT_MAX / 2)
+        return fail(SPC3D_ERR_TOO_LARGE, "a sequence of more than 2^30 - 1 tokens or rows");
+    return SPC3D_OK;
+}
+
+SeqsView view_of(const spc3d_cache_seqs *s)
+{
+    return SeqsView{(const uint32_t *)s->table, (const uint32_t *)s->lens, (const uint32_t *)s->starts, s->nseq,
+                    s->table_stride, s->rows, std::min(s->max_rows, s->rows), s->max_len};
+}
+
+// What either call over a cache checks of itself and of the operand `h`.
+int check_cached(const spc3d_ctx *ctx, const spc3d_cache *cache, const spc3d_cache_seqs *seqs, const char *name,
+                 const spc3d_heads *h)
+{
+    if (!live(ctx))
+        return fail(SPC3D_ERR_INVALID_ARG, "context is NULL or destroyed");
+    if (!live(cache))
+        return fail(SPC3D_ERR_INVALID_ARG, "cache is NULL or destroyed");
+    if (cache->ctx != ctx)
+        return fail(SPC3D_ERR_INVALID_ARG, "cache belongs to another context");
+    if (int rc = check_seqs(seqs))
+        return rc;
+    if (!h || !live(h->panel))
+        return bad_heads(name, "NULL, or its panel is destroyed");
+    const int dt = h->panel->dtype;
+    if (dt != SPC3D_BF16 && dt != SPC3D_F16)
+        return bad_heads(name, "operands of a cache are bfloat16 or half");
+    if (cache->view.dtype != SPC3D_F8 && cache->view.dtype != dt)
+        return bad_heads(name, "its type is not the cache's", SPC3D_ERR_SIZE_MISMATCH);
+    return check_heads(ctx, name, h, seqs->rows, dt, cache->view.dim);
+}
+
+bool in_cache(const spc3d_cache *c, const spc3d_heads *h)
+{
+    const size_t units = (size_t)c->view.npages * c->view.heads;
+    const size_t bytes = units * c->view.page * c->view.dim * elem_size(c->view.dtype);
+    const void *const p = h->panel->dev;
+    const size_t n = panel_bytes(h->panel);
+    return ranges_overlap(p, n, c->view.k, bytes) || ranges_overlap(p, n, c->view.v, bytes) ||
+           (c->view.k_scale && (ranges_overlap(p, n, c->view.k_scale, 4 * units) ||
+                                ranges_overlap(p, n, c->view.v_scale, 4 * units)));
+}
+
+} // namespace
+
+int spc3d_cache_create(spc3d_ctx *ctx, int dtype, uint32_t npages, uint32_t page, uint32_t heads, uint32_t dim,
+                       spc3d_cache **out)
+{
+    return make_cache(ctx, dtype, npages, page, heads, dim, nullptr, out);
+}
+
+int spc3d_cache_wrap(spc3d_ctx *ctx, int dtype, uint32_t npages, uint32_t page, uint32_t heads, uint32_t dim, void *k,
+                     void *v, void *k_scale, void *v_scale, spc3d_cache **out)
+{
+    void *const mem[4] = {k, v, k_scale, v_scale};
+    return make_cache(ctx, dtype, npages, page, heads, dim, mem, out);
+}
+
+int spc3d_cache_destroy(spc3d_cache *c)
+{
+    if (!live(c))
+        return fail(SPC3D_ERR_INVALID_ARG, "cache is NULL or destroyed");
+    if (int rc = refuse_while_capturing(c->ctx))
+        return rc;
+    (void)hipSetDevice(c->ctx->device);
+    (void)hipStreamSynchronize(c->ctx->stream);
+    if (c->owned)
+        for (void *p : {(void *)c->view.k, (void *)c->view.v, (void *)c->view.k_scale, (void *)c->view.v_scale})
+            if (p) (void)hipFree(p);
+    if (c->work) ctx_free(c->ctx, c->work);
+    for (void *p : c->retired)
+        ctx_free(c->ctx, p);
+    c->magic = 0;
+    delete c;
+    return SPC3D_OK;
+}
+
+int spc3d_cache_device_ptrs(spc3d_cache *c, void **k, void **v, void **k_scale, void **v_scale)
+{
+    if (!live(c))
+        return fail(SPC3D_ERR_INVALID_ARG, "cache is NULL or destroyed");
+    if (k) *k = c->view.k;
+    if (v) *v = c->view.v;
+    if (k_scale) *k_scale = c->view.k_scale;
+    if (v_scale) *v_scale = c->view.v_scale;
+    return SPC3D_OK;
+}
+
+int spc3d_cache_append(spc3d_ctx *ctx, spc3d_cache *cache, const spc3d_cache_seqs *seqs, const spc3d_heads *k,
+                       const spc3d_heads *v, const spc3d_panel *rotations, const spc3d_heads *q,
+                       const spc3d_heads *q_out)
+{
+    int rc = check_cached(ctx, cache, seqs, "k", k);
+    if (rc)
+        return rc;
+    const int dt = k->panel->dtype;
+    const uint32_t dim = cache->view.dim;
+    rc = check_heads(ctx, "v", v, seqs->rows, dt, dim);
+    if (rc)
+        return rc;
+    if (k->heads != cache->view.heads || v->heads != cache->view.heads)
+        return fail(SPC3D_ERR_SIZE_MISMATCH, "k and v need as many heads as the cache");
+    if (!q != !q_out)
+        return fail(SPC3D_ERR_INVALID_ARG, "q and q_out come together");
+    if (q) {
+        rc = check_heads(ctx, "q", q, seqs->rows, dt, dim);
+        if (!rc) rc = check_heads(ctx, "q_out", q_out, seqs->rows, dt, dim);
+        if (rc)
+            return rc;
+        if (q->heads != q_out->heads)
+            return fail(SPC3D_ERR_SIZE_MISMATCH, "q_out needs as many heads as q");
+        if (overlap(q_out, q) || overlap(q_out, k) || overlap(q_out, v))
+            return fail(SPC3D_ERR_INVALID_ARG, "q_out overlaps q, k or v");
+        if (in_cache(cache, q_out))
+            return fail(SPC3D_ERR_INVALID_ARG, "q_out overlaps the cache");
+    }
+    if (in_cache(cache, k) || in_cache(cache, v) || (q && in_cache(cache, q)))
+        return fail(SPC3D_ERR_INVALID_ARG, "an operand overlaps the cache");
+    if (rotations) {
+        if (!live(rotations) || rotations->ctx != ctx)
+            return fail(SPC3D_ERR_INVALID_ARG, "rotations is destroyed or belongs to another context");
+        if (rotations->dtype != SPC3D_F32 || rotations->m < seqs->max_len || rotations->n > dim)
+            return fail(SPC3D_ERR_SIZE_MISMATCH,
+                        "rotations needs a row of floats for every position, no longer than a head");
+        if (rotations->n % 16)
+            return fail(SPC3D_ERR_INVALID_ARG, "a multiple of 16 elements of a head is rotated");
+        if (q_out && ranges_overlap(rotations->dev, panel_bytes(rotations), q_out->panel->dev, panel_bytes(q_out->panel)))
+            return fail(SPC3D_ERR_INVALID_ARG, "q_out overlaps rotations");
+    }
+    AppendArgs a = {};
+    a.c = cache->view;
+    a.s = view_of(seqs);
+    const uint64_t pages = (uint64_t)seqs->nseq * ((a.s.max_rows + a.c.page - 2) / a.c.page + 1) * a.c.heads * 2;
+    if (pages + seqs->rows > INT_MAX)
+        return fail(SPC3D_ERR_TOO_LARGE, "more pages and rows than a grid holds");
+    rc = use_device(ctx, true);
+    if (rc)
+        return rc;
+    a.k = view_of(k);
+    a.v = view_of(v);
+    if (q) {
+        a.q = view_of(q);
+        a.q_out = view_of(q_out);
+        a.q_heads = q->heads;
+    }
+    if (rotations && rotations->n) {
+        a.rotations = (const float *)rotations->dev;
+        a.turned = rotations->n;
+    }
+    a.dtype = dt;
+    HIP_TRY(launch_cache_append(a, ctx->stream));
+    return SPC3D_OK;
+}
+
+int spc3d_cache_attend(spc3d_ctx *ctx, spc3d_cache *cache, const spc3d_cache_seqs *seqs, const spc3d_heads *q,
+                       float scale, uint32_t window, uint32_t sinks, const spc3d_heads *o, spc3d_vals *lse)
+{
+    int rc = check_cached(ctx, cache, seqs, "q", q);
+    if (rc)
+        return rc;
+    if (!(scale > 0) || !std::isfinite(scale))
+        return fail(SPC3D_ERR_INVALID_ARG, "scale must be positive and finite");
+    rc = check_heads(ctx, "o", o, seqs->rows, q->panel->dtype, cache->view.dim);
+    if (!rc && lse) rc = check_lse(ctx, lse, (uint64_t)seqs->rows * q->heads);
+    if (rc)
+        return rc;
+    if (q->heads % cache->view.heads || o->heads != q->heads)
+        return fail(SPC3D_ERR_SIZE_MISMATCH, "q needs a multiple of the cache's heads, o as many as q");
+    if (overlap(o, q) || in_cache(cache, o))
+        return fail(SPC3D_ERR_INVALID_ARG, "o overlaps q or the cache");
+    ReadArgs a = {};
+    a.c = cache->view;
+    a.s = view_of(seqs);
+    a.q = view_of(q);
+    a.o = view_of(o);
+    a.lse = lse ? (float *)lse->dev : nullptr;
+    a.heads = q->heads;
+    a.window = window && window < (uint32_t)INT_MAX ? (int32_t)window : INT_MAX;
+    a.sinks = window ? (int32_t)std::min(sinks, (uint32_t)INT_MAX / 2) : 0;
+    a.scale = scale;
+    a.dtype = q->panel->dtype;
+    const uint32_t group = q->heads / a.c.heads, cols = read_columns(a.s.max_rows, group);
+    const uint64_t tiles = ((uint64_t)a.s.max_rows * group + cols - 1) / cols;
+    const uint64_t groups = (uint64_t)seqs->nseq * tiles * a.c.heads;
+    // Workgroups for two on each CU, as far as each gets two steps of 64 tokens for every one of
+    // its four wavefronts.
+    uint64_t steps = ((uint64_t)seqs->max_len + kKeyStep - 1) / kKeyStep;
+    if (a.window != INT_MAX)
+        steps = std::min(steps, ((uint64_t)window + a.s.max_rows + kKeyStep - 1) / kKeyStep + 1 +
+                                    ((uint64_t)a.sinks + kKeyStep - 1) / kKeyStep);
+    const uint64_t want = 2ull * ctx->cu_count;
+    a.splits = 1;
+    if (groups && groups < want)
+        a.splits = (uint32_t)std::max<uint64_t>(1, std::min((want + groups - 1) / groups, steps / 8));
+    a.col_tiles = (uint32_t)tiles;
+    if (groups * a.splits > INT_MAX || (uint64_t)seqs->rows * q->heads / 8 > INT_MAX)
+        return fail(SPC3D_ERR_TOO_LARGE, "more rows and heads than a grid holds");
+    rc = use_device(ctx, true);
+    if (rc)
+        return rc;
+    if (a.splits > 1) {
+        rc = ensure_work(cache, (uint64_t)seqs->rows * q->heads * a.splits * (a.c.dim + 4));
+        if (rc)
+            return rc;
+        a.partial = cache->work;
+    }
+    HIP_TRY(launch_cache_read(a, ctx->stream));
     return SPC3D_OK;
 }
 

@@ -63,6 +63,7 @@ constexpr uint32_t kMagicPlan = 0x5343334c;
 constexpr uint32_t kMagicRowMap = 0x5343334d;
 constexpr uint32_t kMagicGraph = 0x53433347;
 constexpr uint32_t kMagicBand = 0x53433342;
+constexpr uint32_t kMagicCache = 0x5343334b;
 constexpr int kTimerSlots = 4096;
 constexpr uint32_t kMaxColBlocks = 4096;
 
@@ -540,6 +541,27 @@ inline bool ranges_overlap(const void *a, size_t abytes, const void *b, size_t b
 inline size_t panel_bytes(const spc3d_panel *p)
 {
     return (size_t)p->m * p->n * elem_size(p->dtype);
+}
+
+// `dev` must be `bytes` of device memory of ctx's GPU, 16-byte aligned (the copy and
+// pack kernels move 16-byte vectors from the start of a buffer).
+inline int check_wrapped(spc3d_ctx *ctx, const void *dev, size_t bytes)
+{
+    if (bytes == 0)
+        return SPC3D_OK;
+    if (!dev)
+        return fail(SPC3D_ERR_INVALID_ARG, "device pointer is NULL");
+    if (reinterpret_cast<uintptr_t>(dev) % 16)
+        return fail(SPC3D_ERR_INVALID_ARG, "device pointer is not 16-byte aligned");
+    hipPointerAttribute_t at;
+    std::memset(&at, 0, sizeof at);
+    if (hipPointerGetAttributes(&at, dev) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(SPC3D_ERR_INVALID_ARG, "pointer is not known to the HIP runtime");
+    }
+    if (at.type != hipMemoryTypeDevice || at.device != ctx->device)
+        return fail(SPC3D_ERR_INVALID_ARG, "pointer is not device memory of the context's GPU");
+    return SPC3D_OK;
 }
 
 // The ordinary parts a call works on: the plan itself, or its column blocks (beside a

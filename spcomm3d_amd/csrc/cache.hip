@@ -1,0 +1,675 @@
+// A paged cache of keys and values: new rows put into it, rotated and rounded on the way, and
+// attention of a few rows over it.
+#include "cache.h"
+#include "attention_frag.h"
+
+namespace spc3d {
+namespace {
+
+constexpr int kThreads = 256;
+
+// What a sequence is, with nothing past what the caller's bounds allow.
+struct Seq {
+    uint32_t row0, n; // its rows
+    int len, first;   // tokens held; position of row row0 (negative: len is less than n)
+};
+__device__ __forceinline__ Seq seq_of(const SeqsView &s, uint32_t b, uint32_t page)
+{
+    Seq q;
+    q.row0 = min(s.starts[b], s.rows);
+    q.n = min(max(min(s.starts[b + 1], s.rows), q.row0) - q.row0, s.max_rows);
+    q.len = (int)min(min((uint64_t)s.lens[b], (uint64_t)s.max_len), (uint64_t)s.table_stride * page);
+    q.first = q.len - (int)q.n;
+    return q;
+}
+
+// ---- append -----------------------------------------------------------------------------------
+// Eight elements from d on of the row at `p`, rotated by the angles of position `pos`: pairs
+// (j, j + turned / 2).  Products and sums are rounded one by one, as the formula is written.
+template <typename T>
+__device__ __forceinline__ f32x8 rotated(const T *p, int d, const float *rotations, int turned, int64_t pos)
+{
+#pragma clang fp contract(off)
+    const Frag<T> x = load_frag(p + d);
+    f32x8 y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        y[j] = (float)x[j];
+    if (!rotations || d >= turned)
+        return y;
+    const int half = turned / 2, at = d < half ? d : d - half;
+    const Frag<T> z = load_frag(p + (d < half ? d + half : d - half));
+    const float *const c = rotations + pos * turned + at;
+    const f32x8 cos = load_frag(c), sin = load_frag(c + half);
+    const float sign = d < half ? -1.0f : 1.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        y[j] = y[j] * cos[j] + sign * ((float)z[j] * sin[j]);
+    return y;
+}
+
+// The smallest 2^e, -40 <= e <= 40, with most <= 448 * 2^e.
+__device__ __forceinline__ float scale_for(float most)
+{
+    const uint32_t bits = __float_as_uint(most);
+    const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000);
+    return __uint_as_float((uint32_t)(min(max(e, -40), 40) + 127) << 23);
+}
+
+__device__ __forceinline__ u32x2 pack_f8(const float *x)
+{
+    u32x2 w;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        int v = __builtin_amdgcn_cvt_pk_fp8_f32(f8_range(x[4 * h]), f8_range(x[4 * h + 1]), 0, false);
+        w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(f8_range(x[4 * h + 2]), f8_range(x[4 * h + 3]), v, true);
+    }
+    return w;
+}
+__device__ __forceinline__ void unpack_f8(u32x2 w, float *x)
+{
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
+        x[4 * h] = a[0];
+        x[4 * h + 1] = a[1];
+        x[4 * h + 2] = b[0];
+        x[4 * h + 3] = b[1];
+    }
+}
+
+// One workgroup has the keys or the values of one page and head to itself, so that a page's scale
+// and the re-rounding of what it holds need no other's word.  C: what the cache holds.
+template <typename T, typename C>
+__device__ __forceinline__ void append_page(const AppendArgs &a, uint32_t b, uint32_t nth, uint32_t head, bool values,
+                                            float *reduce)
+{
+    constexpr bool kF8 = sizeof(C) == 1;
+    const Seq s = seq_of(a.s, b, a.c.page);
+    const int page = (int)a.c.page, dim = (int)a.c.dim, tid = threadIdx.x;
+    const int begin = max(s.first, 0);
+    if (!s.n || begin >= s.len)
+        return;
+    const int p = begin / page + (int)nth;
+    const int lo = max(begin - p * page, 0), hi = min(s.len - p * page, page); // new slots
+    if (lo >= hi)
+        return;
+    const uint32_t id = a.s.table[(uint64_t)b * a.s.table_stride + p];
+    if (id >= a.c.npages)
+        return;
+    const uint64_t unit = (uint64_t)id * a.c.heads + head;
+    const HeadsView &from = values ? a.v : a.k;
+    const T *const src = (const T *)from.p + head * dim;
+    C *const dst = (C *)(values ? a.c.v : a.c.k) + unit * page * dim;
+    const float *const rot = values ? nullptr : a.rotations;
+    // panel row of slot j: row0 + (p page + j - first)
+    const int64_t row0 = (int64_t)s.row0 + (int64_t)p * page - s.first;
+    const int chunks = dim / 8;
+
+    float scale = 1.0f, ratio = 1.0f;
+    if constexpr (kF8) {
+        float most = 0.0f;
+        for (int i = tid; i < (hi - lo) * chunks; i += kThreads) {
+            const int j = lo + i / chunks, d = i % chunks * 8;
+            const f32x8 x = rotated(src + (row0 + j) * from.stride, d, rot, (int)a.turned, (int64_t)p * page + j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (fabsf(x[e]) < __builtin_inff())
+                    most = fmaxf(most, fabsf(x[e]));
+        }
+#pragma unroll
+        for (int m = 32; m; m >>= 1)
+            most = fmaxf(most, __shfl_xor(most, m));
+        if ((tid & 63) == 0)
+            reduce[tid >> 6] = most;
+        float *const held = (values ? a.c.v_scale : a.c.k_scale) + unit;
+        const float before = *held;
+        __syncthreads();
+        scale = scale_for(fmaxf(fmaxf(reduce[0], reduce[1]), fmaxf(reduce[2], reduce[3])));
+        if (lo > 0) { // the page was begun before
+            const float held_by = before > 0 ? before : 0.0f;
+            scale = fmaxf(scale, held_by);
+            ratio = held_by / scale;
+        }
+        if (tid == 0)
+            *held = scale; // every thread has read it
+    }
+    const int from_slot = ratio == 1.0f ? lo : 0; // a larger scale: what the page holds is rounded again
+    if (!values) {
+        for (int i = tid; i < (hi - from_slot) * chunks; i += kThreads) {
+            const int j = from_slot + i / chunks, d = i % chunks * 8;
+            C *const to = dst + j * dim + d;
+            float x[8];
+            if constexpr (kF8) {
+                if (j < lo) {
+                    unpack_f8(*(const u32x2 *)to, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        x[e] *= ratio;
+                } else {
+                    const f32x8 y = rotated(src + (row0 + j) * from.stride, d, rot, (int)a.turned, (int64_t)p * page + j);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        x[e] = y[e] / scale;
+                }
+                *(u32x2 *)to = pack_f8(x);
+            } else {
+                const f32x8 y = rotated(src + (row0 + j) * from.stride, d, rot, (int)a.turned, (int64_t)p * page + j);
+                Frag<C> f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    f[e] = (C)y[e];
+                *(Frag<C> *)to = f;
+            }
+        }
+        return;
+    }
+    // values: eight slots of one element at a time
+    const int first = from_slot / 8, blocks = (hi + 7) / 8 - first;
+    for (int i = tid; i < blocks * dim; i += kThreads) {
+        const int d = i % dim, j0 = (first + i / dim) * 8;
+        C *const to = dst + (uint64_t)d * page + j0;
+        T x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[e] = j0 + e >= lo && j0 + e < hi ? src[(row0 + j0 + e) * (int64_t)from.stride + d] : (T)0.0f;
+        if constexpr (kF8) {
+            float y[8], old[8];
+            const u32x2 was = *(const u32x2 *)to;
+            unpack_f8(was, old);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                y[e] = j0 + e < lo ? old[e] * ratio : (float)x[e] / scale;
+            u32x2 w = pack_f8(y);
+            if (j0 + 8 > hi) { // slots that no token has yet keep what they hold
+                const int keep = hi - j0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int n = min(max(keep - 4 * h, 0), 4);
+                    const uint32_t mask = n == 4 ? 0xffffffffu : (1u << 8 * n) - 1;
+                    w[h] = (w[h] & mask) | (was[h] & ~mask);
+                }
+            }
+            *(u32x2 *)to = w;
+        } else {
+            Frag<C> f = *(const Frag<C> *)to;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (j0 + e >= lo && j0 + e < hi)
+                    f[e] = (C)x[e];
+            *(Frag<C> *)to = f;
+        }
+    }
+}
+
+// The sequence that a row belongs to: the last one that starts at or before it and is not empty.
+__device__ __forceinline__ uint32_t seq_of_row(const SeqsView &s, uint32_t row)
+{
+    uint32_t lo = 0, hi = s.nseq; // starts[lo] <= row < starts[hi], where starts ascend
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (s.starts[mid] <= row)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+template <typename T, typename C> __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, uint32_t per_seq)
+{
+    __shared__ float reduce[kThreads / 64];
+    const uint32_t pages = a.s.nseq * per_seq * a.c.heads * 2;
+    uint32_t id = blockIdx.x;
+    if (id < pages) {
+        const bool values = id & 1;
+        id >>= 1;
+        const uint32_t head = id % a.c.heads;
+        id /= a.c.heads;
+        append_page<T, C>(a, id / per_seq, id % per_seq, head, values, reduce);
+        return;
+    }
+    const uint32_t row = id - pages; // a row of queries
+    const uint32_t b = seq_of_row(a.s, row);
+    const Seq s = seq_of(a.s, b, a.c.page);
+    if (row < s.row0 || row - s.row0 >= s.n)
+        return;
+    const int pos = s.first + (int)(row - s.row0), dim = (int)a.c.dim, chunks = dim / 8;
+    const T *const src = (const T *)a.q.p + row * a.q.stride;
+    T *const dst = (T *)a.q_out.p + row * a.q_out.stride;
+    for (int i = threadIdx.x; i < (int)a.q_heads * chunks; i += kThreads) {
+        const int h = i / chunks, d = i % chunks * 8;
+        const f32x8 y = rotated(src + h * dim, d, pos < 0 ? nullptr : a.rotations, (int)a.turned, pos);
+        Frag<T> f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            f[e] = (T)y[e];
+        *(Frag<T> *)(dst + h * dim + d) = f;
+    }
+}
+
+// ---- read -------------------------------------------------------------------------------------
+// Columns are the (row, head) pairs that share a kv head, 16 NC of them a workgroup; its four
+// wavefronts take 64 tokens at a time, in turn, each with its own running maximum and sum, joined
+// at the end.  Nothing goes through LDS on the way: S^T = K Q^T wants a token's elements, O^T =
+// V^T P^T an element's tokens, and that is how the cache holds them.  Which token stands in which
+// row of S^T is free; they are dealt so that a lane's probabilities are the tokens 16 g .. 16 g + 15
+// of its own group, which is what it loads of V.
+template <typename T, typename C, int DP> struct Loaded {
+    // keys of tile (u, w): elements as the fragments of q are laid out; values: 16 tokens of element 16 n + l
+    static constexpr int kPer = 16 / (int)sizeof(C); // elements of a load
+    static constexpr int KL = DP / (4 * kPer), VL = sizeof(C) == 1 ? 1 : 2;
+    u32x4 k[4][KL], v[DP / 16][VL];
+};
+
+template <typename T> __device__ __forceinline__ Frag<T> from_f8(uint32_t lo, uint32_t hi);
+template <> __device__ __forceinline__ bf16x8 from_f8<bf16_t>(uint32_t lo, uint32_t hi)
+{
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+template <> __device__ __forceinline__ f16x8 from_f8<f16_t>(uint32_t lo, uint32_t hi)
+{
+    typedef uint32_t u32;
+    const u32 a = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+    const u32 b = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+    const u32 c = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+    const u32 d = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+    return __builtin_bit_cast(f16x8, u32x4{a, b, c, d});
+}
+
+__device__ __forceinline__ bool sees(int p, int c, int window, int sinks)
+{
+    return c <= p && (p - c < window || c < sinks);
+}
+
+// Steps of 64 tokens that rows at positions pa .. pb go over (see attention.hip).
+struct Steps {
+    int first, from, count;
+    __device__ __forceinline__ int at(int k) const { return k < first ? k : from + k - first; }
+};
+__device__ __forceinline__ Steps steps_of(int pa, int pb, int len, int window, int sinks)
+{
+    const int end = min(pb + 1, len), step = (int)kKeyStep;
+    Steps s{0, 0, 0};
+    if (end <= 0)
+        return s;
+    const int lo = window > pa ? 0 : pa - window + 1;
+    s.first = (min(sinks, end) + step - 1) / step;
+    s.from = max(lo / step, s.first);
+    s.count = s.first + max(0, (end + step - 1) / step - s.from);
+    return s;
+}
+
+template <typename T, typename C, int DP, int NC>
+__global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
+{
+    constexpr bool kF8 = sizeof(C) == 1;
+    constexpr int NS = DP / 32, ND = DP / 16, COLS = 16 * NC;
+    typedef Loaded<T, C, DP> L;
+    __shared__ float out[4][COLS][DP + 4]; // by wavefront; 4 more: no two columns on the same banks
+    __shared__ float part_m[4][COLS], part_sum[4][COLS];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int dim = (int)a.c.dim, page = (int)a.c.page;
+    const uint32_t group = a.heads / a.c.heads;
+    uint32_t id = blockIdx.x;
+    const uint32_t head = id % a.c.heads;
+    id /= a.c.heads;
+    const uint32_t split = id % a.splits;
+    id /= a.splits;
+    const uint32_t tile = id % a.col_tiles, b = id / a.col_tiles;
+    const Seq s = seq_of(a.s, b, a.c.page);
+    const int cols = (int)(s.n * group), m0 = (int)tile * COLS;
+    if (m0 >= cols)
+        return;
+
+    Frag<T> qf[NC][NS];
+    int pos[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const int m = m0 + 16 * n + l, i = m / (int)group, h = (int)head * (int)group + m % (int)group;
+        pos[n] = m < cols ? s.first + i : -1;
+        const T *const qp = (const T *)a.q.p + (s.row0 + i) * a.q.stride + h * dim;
+#pragma unroll
+        for (int t = 0; t < NS; ++t) {
+            const int d = kF8 ? 64 * (t / 2) + 16 * g + 8 * (t % 2) : 32 * t + 8 * g;
+            qf[n][t] = m < cols && d < dim ? load_frag(qp + d) : zero_frag<T>();
+        }
+    }
+    const int pa = s.first + m0 / (int)group, pb = s.first + (min(m0 + COLS, cols) - 1) / (int)group;
+    const Steps st = steps_of(pa, pb, s.len, a.window, a.sinks);
+    const int each = (st.count + (int)a.splits - 1) / (int)a.splits;
+    const int k0 = (int)split * each, k1 = min(k0 + each, st.count);
+    const uint32_t *const table = a.s.table + (uint64_t)b * a.s.table_stride;
+    const float sc = a.scale * kLog2e;
+
+    f32x4 acc[ND][NC];
+    float m[NC], sum[NC], ref;
+    for (int careful = 0; careful < 2; ++careful) { // see attend_kernel
+        ref = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            m[n] = kNegInf;
+            sum[n] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                acc[d][n] = f32x4{0, 0, 0, 0};
+        }
+        for (int k = k0 + wave; k < k1; k += 4) {
+            const int c0 = st.at(k) * (int)kKeyStep;
+            // pages of the 16 tokens that this lane loads keys of, and values of
+            const int ck = c0 + 16 * (l >> 2), cg = c0 + 16 * g;
+            const uint32_t pk = ck < s.len ? table[ck / page] : a.c.npages;
+            const uint32_t pv = cg < s.len ? table[cg / page] : a.c.npages;
+            const bool in_k = pk < a.c.npages, in_v = pv < a.c.npages;
+            L x;
+            const C *const kp = (const C *)a.c.k + (((uint64_t)(in_k ? pk : 0) * a.c.heads + head) * page + ck % page + (l & 3)) * dim;
+            const C *const vp = (const C *)a.c.v + ((uint64_t)(in_v ? pv : 0) * a.c.heads + head) * page * dim + cg % page;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < L::KL; ++t) {
+                    const int d = t * 4 * L::kPer + g * L::kPer;
+                    x.k[i][t] = u32x4{0, 0, 0, 0};
+                    if (in_k && d < dim)
+                        x.k[i][t] = *(const u32x4 *)(kp + 4 * i * dim + d);
+                }
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int t = 0; t < L::VL; ++t) {
+                    x.v[d][t] = u32x4{0, 0, 0, 0};
+                    if (in_v && 16 * d + l < dim)
+                        x.v[d][t] = *(const u32x4 *)(vp + (uint64_t)(16 * d + l) * page + t * L::kPer);
+                }
+            float ks = sc, vs = 1.0f;
+            if constexpr (kF8) {
+                const uint64_t at = (uint64_t)(in_v ? pv : 0) * a.c.heads + head;
+                ks = sc * a.c.k_scale[at];
+                vs = a.c.v_scale[at];
+            }
+            // Tokens that no row of the tile sees (not there yet, left of the window) may hold
+            // anything: their values become 0.  Edges only, all else is a whole step.
+            const int c9 = c0 + (int)kKeyStep - 1;
+            const bool whole = c9 <= pa && (pb - c0 < a.window || c9 < a.sinks) && __all(in_v);
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < L::VL; ++t)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t mask = 0;
+#pragma unroll
+                        for (int e = 0; e < L::kPer / 4; ++e) {
+                            const int c = cg + t * L::kPer + w * (L::kPer / 4) + e;
+                            const bool seen = in_v && c <= pb && (c < a.sinks || pa - c < a.window);
+                            mask |= seen ? (kF8 ? 0xffu << 8 * e : 0xffffu << 16 * e) : 0;
+                        }
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+                            x.v[d][t][w] &= mask;
+                    }
+                if (!in_v || cg > pb || !(cg < a.sinks || pa - (cg + 15) < a.window))
+                    ks = vs = 0.0f; // a scale that belongs to nothing seen
+            }
+            f32x4 sv[4][NC];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+                    sv[i][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < NS; ++t) {
+                    Frag<T> f;
+                    if constexpr (kF8)
+                        f = from_f8<T>(x.k[i][t / 2][2 * (t % 2)], x.k[i][t / 2][2 * (t % 2) + 1]);
+                    else
+                        f = __builtin_bit_cast(Frag<T>, x.k[i][t]);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n)
+                        sv[i][n] = mma(f, qf[n][t], sv[i][n]);
+                }
+            }
+            // sv[i][n][j]: token cg + 4 i + j
+            float to_ref = 1.0f, weigh = 1.0f;
+            if constexpr (kF8) { // acc is in units of the largest scale of values so far
+                const float top = fmaxf(ref, column_max(fabsf(vs)));
+                to_ref = top > 0 ? ref / top : 0.0f;
+                weigh = top > 0 ? vs / top : vs;
+                ref = top;
+            }
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                float top = kNegInf;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float y = sv[i][n][j] * ks;
+                        if (!whole && !(in_v && sees(pos[n], cg + 4 * i + j, a.window, a.sinks)))
+                            y = kNegInf;
+                        sv[i][n][j] = y;
+                        top = fmaxf(top, y);
+                    }
+                top = fmaxf(m[n], column_max(top));
+                const float base = top == kNegInf ? 0.0f : top;
+                const float down = __builtin_amdgcn_exp2f(m[n] - base), less = base - WeightShift<T>::value;
+                m[n] = top;
+                float add = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = __builtin_amdgcn_exp2f(sv[i][n][j] - less);
+                        add += p;
+                        sv[i][n][j] = kF8 ? p * weigh : p;
+                    }
+                sum[n] = sum[n] * down + add;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    acc[d][n] *= kF8 ? down * to_ref : down;
+            }
+            const bool one_by_one = careful && !whole;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                Frag<T> pf[NC];
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+                    pf[n] = join<T>(sv[2 * u][n], sv[2 * u + 1][n]);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<T> f;
+                    if constexpr (kF8)
+                        f = from_f8<T>(x.v[d][0][2 * u], x.v[d][0][2 * u + 1]);
+                    else
+                        f = __builtin_bit_cast(Frag<T>, x.v[d][u]);
+                    if (one_by_one) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (!(fabsf((float)f[j]) < __builtin_inff()))
+                                f[j] = (T)0.0f;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NC; ++n)
+                        acc[d][n] = mma(f, pf[n], acc[d][n]);
+                }
+            }
+            if (one_by_one) {
+                for (int c = c0; c <= min(c9, pb); ++c) {
+                    const uint32_t pc = table[c / page];
+                    if (pc >= a.c.npages)
+                        continue;
+                    const C *const from = (const C *)a.c.v + ((uint64_t)pc * a.c.heads + head) * page * dim + c % page;
+                    for (int d = 0; d < ND; ++d)
+                        for (int j = 0; j < 4; ++j) {
+                            const int e = 16 * d + 4 * g + j;
+                            if (e >= dim)
+                                continue;
+                            float y;
+                            if constexpr (kF8)
+                                y = __builtin_amdgcn_cvt_pk_f32_fp8((int)from[(uint64_t)e * page], false)[0];
+                            else
+                                y = (float)from[(uint64_t)e * page];
+                            if (fabsf(y) < __builtin_inff())
+                                continue;
+#pragma unroll
+                            for (int n = 0; n < NC; ++n)
+                                if (sees(pos[n], c, a.window, a.sinks)) {
+#pragma unroll
+                                    for (int dd = 0; dd < ND; ++dd) // registers have no run-time number
+#pragma unroll
+                                        for (int jj = 0; jj < 4; ++jj)
+                                            if (dd == d && jj == j)
+                                                acc[dd][n][jj] += y;
+                                }
+                        }
+                }
+            }
+        }
+        bool bad = false;
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    bad |= pos[n] >= 0 && !(fabsf(acc[d][n][j]) < __builtin_inff());
+        if (careful || !__any(bad))
+            break;
+    }
+
+    // the four wavefronts joined, in their order
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        sum[n] = column_sum(sum[n]);
+        if (g == 0) {
+            part_m[wave][16 * n + l] = m[n];
+            part_sum[wave][16 * n + l] = sum[n];
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            *(f32x4 *)&out[wave][16 * n + l][16 * d + 4 * g] = kF8 ? acc[d][n] * ref : acc[d][n];
+    }
+    __syncthreads();
+    constexpr int kQuads = DP / 4;
+    for (int i = tid; i < COLS * kQuads; i += kThreads) {
+        const int c = i / kQuads, d = i % kQuads * 4, mm = m0 + c;
+        if (mm >= cols || d >= dim)
+            continue;
+        float top = part_m[0][c];
+#pragma unroll
+        for (int w = 1; w < 4; ++w)
+            top = fmaxf(top, part_m[w][c]);
+        const float base = top == kNegInf ? 0.0f : top;
+        float total = 0.0f;
+        f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float by = __builtin_amdgcn_exp2f(part_m[w][c] - base);
+            total += part_sum[w][c] * by;
+            y += *(const f32x4 *)&out[w][c][d] * by;
+        }
+        const uint64_t row = s.row0 + mm / (int)group;
+        const uint32_t h = head * group + mm % (int)group;
+        if (a.splits > 1) {
+            float *const to = a.partial + ((row * a.heads + h) * a.splits + split) * (dim + 4);
+            *(f32x4 *)(to + 4 + d) = y;
+            if (d == 0) {
+                to[0] = top;
+                to[1] = total;
+            }
+        } else {
+            const float by = total == 0.0f ? 0.0f : 1.0f / total;
+            store_half<T>((T *)a.o.p + row * a.o.stride + h * dim + d, y * by);
+            if (d == 0 && a.lse)
+                a.lse[row * a.heads + h] = total == 0.0f ? kNegInf : (top + __log2f(total) - WeightShift<T>::value) * kLn2;
+        }
+    }
+}
+
+// The splits of a row and head joined, in their order; a wavefront for each, four elements a lane.
+template <typename T> __global__ __launch_bounds__(kThreads) void read_join_kernel(ReadArgs a)
+{
+    const uint32_t lane = threadIdx.x & 31, dim = a.c.dim;
+    const uint64_t at = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / 32;
+    if (at >= (uint64_t)a.s.rows * a.heads)
+        return;
+    const uint64_t row = at / a.heads;
+    const uint32_t h = (uint32_t)(at % a.heads);
+    const uint32_t b = seq_of_row(a.s, (uint32_t)row);
+    const Seq s = seq_of(a.s, b, a.c.page);
+    if (row < s.row0 || row - s.row0 >= s.n)
+        return;
+    const float *const part = a.partial + at * a.splits * (dim + 4);
+    float top = kNegInf;
+    for (uint32_t i = 0; i < a.splits; ++i)
+        top = fmaxf(top, part[i * (dim + 4)]);
+    const float base = top == kNegInf ? 0.0f : top;
+    float total = 0.0f;
+    f32x4 y = {0, 0, 0, 0};
+    for (uint32_t i = 0; i < a.splits; ++i) {
+        const float *const p = part + i * (dim + 4);
+        const float by = __builtin_amdgcn_exp2f(p[0] - base);
+        total += p[1] * by;
+        if (4 * lane < dim)
+            y += *(const f32x4 *)(p + 4 + 4 * lane) * by;
+    }
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    if (4 * lane < dim)
+        store_half<T>((T *)a.o.p + row * a.o.stride + h * dim + 4 * lane, y * by);
+    if (lane == 0 && a.lse)
+        a.lse[at] = total == 0.0f ? kNegInf : (top + __log2f(total) - WeightShift<T>::value) * kLn2;
+}
+
+template <typename T, typename C, int DP> hipError_t launch_read_one(const ReadArgs &a, hipStream_t s)
+{
+    const dim3 grid(a.s.nseq * a.col_tiles * a.splits * a.c.heads), block(kThreads);
+    if (read_columns(a.s.max_rows, a.heads / a.c.heads) == 16)
+        hipLaunchKernelGGL((read_kernel<T, C, DP, 1>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((read_kernel<T, C, DP, 2>), grid, block, 0, s, a);
+    if (a.splits > 1) {
+        const uint64_t all = (uint64_t)a.s.rows * a.heads * 32;
+        hipLaunchKernelGGL((read_join_kernel<T>), dim3((uint32_t)((all + kThreads - 1) / kThreads)), block, 0, s, a);
+    }
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_read(const ReadArgs &a, hipStream_t s)
+{
+    if (a.c.dtype == 4)
+        return a.c.dim <= 64 ? launch_read_one<T, uint8_t, 64>(a, s) : launch_read_one<T, uint8_t, 128>(a, s);
+    return a.c.dim <= 64 ? launch_read_one<T, T, 64>(a, s) : launch_read_one<T, T, 128>(a, s);
+}
+
+template <typename T> hipError_t launch_append(const AppendArgs &a, hipStream_t s)
+{
+    const uint32_t per_seq = (a.s.max_rows + a.c.page - 2) / a.c.page + 1; // pages that so many rows touch
+    const uint64_t grid = (uint64_t)a.s.nseq * per_seq * a.c.heads * 2 + (a.q.p ? a.s.rows : 0);
+    if (a.c.dtype == 4)
+        hipLaunchKernelGGL((append_kernel<T, uint8_t>), dim3((uint32_t)grid), dim3(kThreads), 0, s, a, per_seq);
+    else
+        hipLaunchKernelGGL((append_kernel<T, T>), dim3((uint32_t)grid), dim3(kThreads), 0, s, a, per_seq);
+    return hipGetLastError();
+}
+
+} // namespace
+
+uint32_t read_columns(uint32_t max_rows, uint32_t group) { return (uint64_t)max_rows * group <= 16 ? 16 : 32; }
+
+hipError_t launch_cache_append(const AppendArgs &a, hipStream_t stream)
+{
+    if (!a.s.nseq || !a.s.rows || !a.s.max_rows)
+        return hipSuccess;
+    return a.dtype == 2 ? launch_append<bf16_t>(a, stream) : launch_append<f16_t>(a, stream);
+}
+
+hipError_t launch_cache_read(const ReadArgs &a, hipStream_t stream)
+{
+    if (!a.s.nseq || !a.s.rows || !a.s.max_rows)
+        return hipSuccess;
+    return a.dtype == 2 ? launch_read<bf16_t>(a, stream) : launch_read<f16_t>(a, stream);
+}
+
+} // namespace spc3d

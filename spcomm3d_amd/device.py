@@ -188,6 +188,11 @@ class Context:
         seeing the last ``window`` columns up to its own (0: all) and the first ``sinks``."""
         return Band(self, rows, cols, window, sinks)
 
+    def cache(self, dtype: str, pages: int, page: int, heads: int, dim: int, k: int | None = None,
+              v: int | None = None, k_scale: int | None = None, v_scale: int | None = None) -> "Cache":
+        """``pages`` pages of ``page`` tokens in ``"bf16"``, ``"f16"`` or ``"f8"`` (:class:`Cache`)."""
+        return Cache(self, dtype, pages, page, heads, dim, k, v, k_scale, v_scale)
+
     def attend(self, band: "Band", q: "Heads", k: "Heads", v: "Heads", o: "Heads",
                lse: "Vals | None" = None, scale: float | None = None):
         """o = softmax(scale q k^T) v over the band (``spc3d_attend``); ``scale``: 1 / sqrt(dim)
@@ -331,6 +336,77 @@ class Band:
     def close(self):
         if getattr(self, "_h", None) and getattr(self.ctx, "_h", None):
             self.ctx._lib.spc3d_band_destroy(self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class CacheSeqs:
+    """The sequences of a call over a cache (``spc3d_cache_seqs``): device addresses of the page
+    table (``table_stride`` entries a sequence), the lengths and the first rows, and the bounds
+    that launches are sized for."""
+
+    def __init__(self, nseq: int, table: int, table_stride: int, lens: int, starts: int, rows: int,
+                 max_rows: int, max_len: int):
+        self._arg = capi.CacheSeqsArg(int(nseq), int(table_stride), int(rows), int(max_rows), int(max_len), 0,
+                                      table, lens, starts)
+        self._ref = ctypes.byref(self._arg)
+
+
+class Cache:
+    """Keys and values of growing sequences in pages (``spc3d_cache``)."""
+
+    def __init__(self, ctx: Context, dtype: str, pages: int, page: int, heads: int, dim: int,
+                 k: int | None = None, v: int | None = None, k_scale: int | None = None,
+                 v_scale: int | None = None):
+        """``k``, ``v`` and, in 8 bits, the scales: device addresses to wrap
+        (``spc3d_cache_wrap``) instead of allocating."""
+        self.ctx, self.dtype = ctx, dtype
+        self.pages, self.page, self.heads, self.dim = int(pages), int(page), int(heads), int(dim)
+        code = _SHORT[dtype][0] if dtype in _SHORT else dtype_code(dtype)
+        h = ctypes.c_void_p()
+        if k is None and v is None:
+            check(ctx._lib.spc3d_cache_create(ctx._h, code, self.pages, self.page, self.heads, self.dim,
+                                              ctypes.byref(h)), "spc3d_cache_create")
+        else:
+            check(ctx._lib.spc3d_cache_wrap(ctx._h, code, self.pages, self.page, self.heads, self.dim, k, v,
+                                            k_scale, v_scale, ctypes.byref(h)), "spc3d_cache_wrap")
+        self._h = h
+
+    def device_ptrs(self) -> tuple[int, int, int, int]:
+        """Addresses of keys, values and their scales (0: none)."""
+        p = [ctypes.c_void_p() for _ in range(4)]
+        check(self.ctx._lib.spc3d_cache_device_ptrs(self._h, *(ctypes.byref(x) for x in p)),
+              "spc3d_cache_device_ptrs")
+        return tuple(x.value or 0 for x in p)
+
+    def append(self, seqs: CacheSeqs, k: Heads, v: Heads, rotations: Panel | None = None,
+               q: Heads | None = None, q_out: Heads | None = None):
+        """The newest rows of every sequence go to the cache, keys (and ``q`` on its way to
+        ``q_out``) rotated by their positions' angles (``spc3d_cache_append``); asynchronous."""
+        rc = self.ctx._lib.spc3d_cache_append(
+            self.ctx._h, self._h, seqs._ref, k._ref, v._ref, None if rotations is None else rotations._h,
+            None if q is None else q._ref, None if q_out is None else q_out._ref)
+        if rc:
+            check(rc, "spc3d_cache_append")
+
+    def attend(self, seqs: CacheSeqs, q: Heads, o: Heads, window: int = 0, sinks: int = 0,
+               lse: "Vals | None" = None, scale: float | None = None):
+        """Attention of every sequence's newest rows over what it holds
+        (``spc3d_cache_attend``); ``scale``: 1 / sqrt(dim) unless given; asynchronous."""
+        rc = self.ctx._lib.spc3d_cache_attend(
+            self.ctx._h, self._h, seqs._ref, q._ref, q.dim ** -0.5 if scale is None else scale, window, sinks,
+            o._ref, None if lse is None else lse._h)
+        if rc:
+            check(rc, "spc3d_cache_attend")
+
+    def close(self):
+        if getattr(self, "_h", None) and getattr(self.ctx, "_h", None):
+            self.ctx._lib.spc3d_cache_destroy(self._h)
         self._h = None
 
     def __del__(self):

@@ -103,3 +103,106 @@ def worst(got, want):
     with np.errstate(invalid="ignore"):
         x = np.where(same, 0.0, np.abs(got - value) / bound)
     return float(np.max(np.where(np.isnan(x), np.inf, x), initial=0.0))
+
+
+# ---- 8 bits (e4m3) and the paged cache ------------------------------------------------------
+def _f8_table():
+    t = np.zeros(256)
+    for c in range(256):
+        e, m = (c >> 3) & 15, c & 7
+        x = m / 8 * 2.0 ** -6 if e == 0 else (1 + m / 8) * 2.0 ** (e - 7)
+        t[c] = np.nan if (c & 127) == 127 else x
+        if c & 128:
+            t[c] = -t[c]
+    return t
+
+
+F8 = _f8_table()
+
+
+def f8_codes(x):
+    """To nearest, ties to the even code; beyond 448 that; NaN stays (any of its two codes)."""
+    x = np.asarray(x, dtype=np.float64)
+    up = F8[:127]  # ascending from 0 to 448
+    a = np.minimum(np.where(np.isnan(x), 0.0, np.abs(x)), 448.0)
+    hi = np.clip(np.searchsorted(up, a), 0, 126)
+    lo = np.maximum(hi - 1, 0)
+    dl, dh = a - up[lo], up[hi] - a
+    code = np.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, hi)
+    code = np.where(np.isnan(x), 127, code)
+    return (code + np.where(np.signbit(x), 128, 0)).astype(np.uint8)
+
+
+def scale_for(most):
+    """The smallest 2^e, -40 <= e <= 40, with most <= 448 * 2^e."""
+    e = -40
+    while e < 40 and float(most) > 448.0 * 2.0 ** e:
+        e += 1
+    return np.float32(2.0 ** e)
+
+
+def rotate(x, table, pos):
+    """x [rows, heads, dim] float32, rounded after every operation as the formula is written."""
+    n = table.shape[1]
+    h = n // 2
+    y = x.astype(np.float32).copy()
+    for r, p in enumerate(pos):
+        if p < 0:
+            continue
+        c, s = table[p, :h], table[p, h:]
+        a, b = x[r, :, :h].astype(np.float32), x[r, :, h:n].astype(np.float32)
+        y[r, :, :h] = a * c - b * s
+        y[r, :, h:n] = b * c + a * s
+    return y
+
+
+class HostCache:
+    """The pages of a cache as the library lays them out, on the host."""
+
+    def __init__(self, dtype, pages, page, heads, dim):
+        self.dtype, self.pages, self.page, self.heads, self.dim = dtype, pages, page, heads, dim
+        kind = {"f8": np.uint8, "f16": np.float16, "bf16": np.uint16}[dtype]
+        garbage = {"f8": 0x7F, "f16": np.nan, "bf16": 0x7FC0}[dtype]  # not-a-number until written
+        self.k = np.full((pages, heads, page, dim), garbage, kind)
+        self.v = np.full((pages, heads, dim, page), garbage, kind)
+        self.k_scale = np.full((pages, heads), np.nan, np.float32)
+        self.v_scale = np.full((pages, heads), np.nan, np.float32)
+
+    def append(self, pages_of, first, k, v):
+        """Rows k / v [n, heads, dim] float32 (rotated) at positions first .. of one sequence."""
+        for h in range(self.heads):
+            for p in range(first // self.page, (first + len(k) - 1) // self.page + 1 if len(k) else 0):
+                lo, hi = max(first - p * self.page, 0), min(first + len(k) - p * self.page, self.page)
+                rows = slice(lo + p * self.page - first, hi + p * self.page - first)
+                at = pages_of[p]
+                if at >= self.pages:
+                    continue
+                for held, scales, x in ((self.k[at, h], self.k_scale, k[rows, h]),
+                                        (self.v[at, h].T, self.v_scale, v[rows, h])):
+                    if self.dtype != "f8":
+                        held[lo:hi] = to_bits(x, self.dtype)
+                        continue
+                    with np.errstate(invalid="ignore"):
+                        finite = np.where(np.isfinite(x), np.abs(x), 0)
+                    scale, was = scale_for(finite.max()), scales[at, h]
+                    if lo:
+                        was = was if was > 0 else np.float32(0)
+                        scale = max(scale, was)
+                        if was != scale:
+                            held[:lo] = f8_codes(F8[held[:lo]] * (was / scale))
+                    scales[at, h] = scale
+                    held[lo:hi] = f8_codes(x / scale)
+
+    def values(self, pages_of, n):
+        """Keys and values [n, heads, dim] in 64 bits of a sequence of n tokens."""
+        k, v = np.zeros((n, self.heads, self.dim)), np.zeros((n, self.heads, self.dim))
+        for p in range(-(-n // self.page)):
+            at, hi = pages_of[p], min(self.page, n - p * self.page)
+            if at >= self.pages:
+                continue
+            rows = slice(p * self.page, p * self.page + hi)
+            for out, held, scales in ((k, self.k[at], self.k_scale), (v, self.v[at].transpose(0, 2, 1), self.v_scale)):
+                x = held[:, :hi]
+                x = F8[x] * scales[at].astype(np.float64)[:, None, None] if self.dtype == "f8" else from_bits(x, self.dtype)
+                out[rows] = x.transpose(1, 0, 2)
+        return k, v
