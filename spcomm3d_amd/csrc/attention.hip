@@ -11,6 +11,7 @@ namespace spc3d {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kFewSteps = 2;
 
 struct Work {
     uint32_t tile, head;
@@ -293,85 +294,96 @@ __global__ __launch_bounds__(kThreads, 1) void attend_dq_kernel(BandArgs a)
                 dot = __builtin_fmaf((float)gf[n][s][j], (float)of[j], dot);
         }
         delta[n] = column_sum(dot);
-        const uint64_t at = (uint64_t)(t.row0 + r) * a.heads + w.head;
-        lse[n] = mine ? a.lse[at] * kLog2e : kNegInf;
+        lse[n] = mine ? a.lse[(uint64_t)(t.row0 + r) * a.heads + w.head] * kLog2e : kNegInf;
         if (lse[n] == kNegInf)
             lse[n] = -kNegInf; // a row that sees nothing: every weight is exp2(-inf)
-        if (mine && g == 0)
-            a.delta[at] = delta[n];
     }
     const Steps st = steps_of(t.pos0, t.pos0 + (int)t.nrow - 1, ncols, a.window, a.sinks);
     const int wa = t.pos0 + wave * NQ * 16, wb = min(wa + NQ * 16, t.pos0 + (int)t.nrow) - 1;
     const float sc = a.scale * kLog2e;
 
     f32x4 acc[ND][NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-            acc[d][n] = f32x4{0, 0, 0, 0};
     TileCopy<T, DP, kKeyStep, kThreads> ck, cv;
-    if (st.count > 0) {
-        const int c0 = st.at(0) * (int)kKeyStep;
-        ck.load(kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, tid);
-        cv.load(vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, tid);
-    }
-    for (int k = 0; k < st.count; ++k) {
-        const int c0 = st.at(k) * (int)kKeyStep;
-        __syncthreads();
-        ck.store(kt, tid);
-        cv.store(vt, tid);
-        __syncthreads();
-        if (k + 1 < st.count) {
-            const int c1 = st.at(k + 1) * (int)kKeyStep;
-            ck.load(kp + c1 * a.k.stride, a.k.stride, ncols - c1, dim, tid);
-            cv.load(vp + c1 * a.v.stride, a.v.stride, ncols - c1, dim, tid);
+    float weighed[NQ]; // sum of P dP: <dO, o> again, without the rounding of o
+    // Rows that see few columns take it before they use it: their dS is a small difference, and
+    // the rounding of o in <dO, o> would show (dQ of 300 rows in bfloat16: 1.72 times the error of
+    // one rounding, 1.47 so; further down the sequence it is lost among the columns).
+    for (int last = st.count > kFewSteps; last < 2; ++last) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            weighed[n] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                acc[d][n] = f32x4{0, 0, 0, 0};
         }
-        const int c9 = c0 + (int)kKeyStep - 1;
-        if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
-            continue;
-        const bool whole = c9 <= wa && (wb - c0 < a.window || c9 < a.sinks);
+        if (st.count > 0) {
+            const int c0 = st.at(0) * (int)kKeyStep;
+            ck.load(kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, tid);
+            cv.load(vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, tid);
+        }
+        for (int k = 0; k < st.count; ++k) {
+            const int c0 = st.at(k) * (int)kKeyStep;
+            __syncthreads();
+            ck.store(kt, tid);
+            cv.store(vt, tid);
+            __syncthreads();
+            if (k + 1 < st.count) {
+                const int c1 = st.at(k + 1) * (int)kKeyStep;
+                ck.load(kp + c1 * a.k.stride, a.k.stride, ncols - c1, dim, tid);
+                cv.load(vp + c1 * a.v.stride, a.v.stride, ncols - c1, dim, tid);
+            }
+            const int c9 = c0 + (int)kKeyStep - 1;
+            if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
+                continue;
+            const bool whole = c9 <= wa && (wb - c0 < a.window || c9 < a.sinks);
 #pragma unroll
-        for (int u = 0; u < NT / 2; ++u) {
-            f32x4 sv[2][NQ], dp[2][NQ];
+            for (int u = 0; u < NT / 2; ++u) {
+                f32x4 sv[2][NQ], dp[2][NQ];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
-                    sv[i][n] = dp[i][n] = f32x4{0, 0, 0, 0};
+                    for (int n = 0; n < NQ; ++n)
+                        sv[i][n] = dp[i][n] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    const Frag<T> f = L::rows(kt, 32 * u + 16 * i, s, lane);
-                    const Frag<T> h = L::rows(vt, 32 * u + 16 * i, s, lane);
+                    for (int s = 0; s < NS; ++s) {
+                        const Frag<T> f = L::rows(kt, 32 * u + 16 * i, s, lane);
+                        const Frag<T> h = L::rows(vt, 32 * u + 16 * i, s, lane);
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        sv[i][n] = mma(f, qf[n][s], sv[i][n]);
-                        dp[i][n] = mma(h, gf[n][s], dp[i][n]);
+                        for (int n = 0; n < NQ; ++n) {
+                            sv[i][n] = mma(f, qf[n][s], sv[i][n]);
+                            dp[i][n] = mma(h, gf[n][s], dp[i][n]);
+                        }
                     }
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i][n][j], sc, -lse[n]));
+                            float y = dp[i][n][j];
+                            if (!whole && !sees(pos[n], c0 + 32 * u + 16 * i + 4 * g + j, a.window, a.sinks))
+                                p = y = 0.0f;
+                            weighed[n] = __builtin_fmaf(p, y, weighed[n]);
+                            sv[i][n][j] = p * (y - delta[n]);
+                        }
                 }
+                if (!last)
+                    continue;
+                Frag<T> df[NQ];
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
+                    df[n] = join<T>(sv[0][n], sv[1][n]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i][n][j], sc, -lse[n]));
-                        float ds = p * (dp[i][n][j] - delta[n]);
-                        if (!whole && !sees(pos[n], c0 + 32 * u + 16 * i + 4 * g + j, a.window, a.sinks))
-                            ds = 0.0f;
-                        sv[i][n][j] = ds;
-                    }
-            }
-            Frag<T> df[NQ];
+                for (int d = 0; d < ND; ++d) {
+                    const Frag<T> f = L::columns(kt, 32 * u, d, lane);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
-                df[n] = join<T>(sv[0][n], sv[1][n]);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const Frag<T> f = L::columns(kt, 32 * u, d, lane);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-                    acc[d][n] = mma(f, df[n], acc[d][n]);
+                    for (int n = 0; n < NQ; ++n)
+                        acc[d][n] = mma(f, df[n], acc[d][n]);
+                }
             }
         }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+            delta[n] = column_sum(weighed[n]);
     }
     T *const dqp = (T *)a.dq.p + t.row0 * a.dq.stride + w.head * dim;
 #pragma unroll
@@ -383,6 +395,8 @@ __global__ __launch_bounds__(kThreads, 1) void attend_dq_kernel(BandArgs a)
         for (int d = 0; d < ND; ++d)
             if (16 * d + 4 * g < dim)
                 store_half<T>(dqp + r * a.dq.stride + 16 * d + 4 * g, acc[d][n] * a.scale);
+        if (g == 0)
+            a.delta[(uint64_t)(t.row0 + r) * a.heads + w.head] = delta[n];
     }
 }
 
