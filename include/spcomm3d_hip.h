@@ -566,7 +566,8 @@ SPC3D_API int spc3d_host_call_stats(spc3d_ctx *ctx, uint64_t *bytes_sent, uint64
  * row t, so q, k and v may lie side by side in one panel.  Panels are SPC3D_F32, SPC3D_BF16 or
  * SPC3D_F16, all of a call the same; sums and softmax statistics are 32-bit; the weights P and
  * dS are rounded once to the panels' type for the second product, results once at the end.
- * dim is a multiple of 8, at most 128; a panel's rows and `col` are whole 16-byte vectors.  The
+ * dim is a multiple of 8, at most 128; a panel's rows (at most 2^22 columns) and `col` are whole
+ * 16-byte vectors.  The
  * heads of q are a multiple of those of k and v: head h reads head h / (heads / kv heads).
  *
  * The sequences lie one after the other: rows rows[0] + .. + rows[b-1] on of q, o and their

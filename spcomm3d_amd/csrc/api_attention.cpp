@@ -28,7 +28,7 @@ struct spc3d_band {
     RowTile *tiles[2] = {nullptr, nullptr}; // of 64 and of 128 rows, the longest walk first
     uint32_t ntiles[2] = {0, 0};
     std::vector<KeySchedule> schedules;
-    // spc3d_attend_grad's workspace: sums <dO, o> of every row and head, partial dK and dV.  A
+    // spc3d_attend_grad's workspace: lse and <dO, o> of every row and head, partial dK and dV.  A
     // block that a call with more heads replaces stays until the band goes: a recorded sequence
     // may use it.
     float *work = nullptr;
@@ -140,7 +140,7 @@ void key_pieces(const spc3d_band *b, uint32_t kv_heads, std::vector<KeyPiece> &p
         key0 += (uint32_t)m;
     }
     const uint64_t want = std::max<uint64_t>(1, 4ull * b->ctx->cu_count / kv_heads);
-    const uint32_t most = (uint32_t)((std::max<uint64_t>(128, (total + want - 1) / want) + 31) / 32 * 32);
+    const uint32_t most = (uint32_t)((std::max<uint64_t>(128, (total + want - 1) / want) + 63) / 64 * 64);
     uint32_t slots = 0;
     for (const KeyPiece &t : tiles) {
         const uint32_t count = (t.nrow + most - 1) / most;
@@ -148,7 +148,7 @@ void key_pieces(const spc3d_band *b, uint32_t kv_heads, std::vector<KeyPiece> &p
             pieces.push_back(t);
             continue;
         }
-        const uint32_t each = ((t.nrow + count - 1) / count + 31) / 32 * 32;
+        const uint32_t each = ((t.nrow + count - 1) / count + 63) / 64 * 64;
         KeySplit sp = {t.key0, t.nkey, slots, 0};
         for (uint32_t r = 0; r < t.nrow; r += each) {
             KeyPiece p = t;
@@ -253,6 +253,8 @@ int check_heads(const spc3d_ctx *ctx, const char *name, const spc3d_heads *h, ui
     const size_t w = elem_size(p->dtype);
     if (p->n * w % 16 || h->col * w % 16)
         return bad_heads(name, "its rows or its first column are no whole 16-byte vectors");
+    if (p->n > 1u << 22)
+        return bad_heads(name, "its panel has more than 2^22 columns", SPC3D_ERR_TOO_LARGE);
     if (p->m < rows)
         return bad_heads(name, "its panel has fewer rows than the sequences", SPC3D_ERR_SIZE_MISMATCH);
     return SPC3D_OK;
@@ -459,8 +461,8 @@ int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q, co
         return rc;
     if ((uint64_t)s->npieces * k->heads > INT_MAX || s->nsplits > INT_MAX || k->heads > 65535)
         return fail(SPC3D_ERR_TOO_LARGE, "more tiles of columns and heads than a grid holds");
-    const uint64_t deltas = ((uint64_t)band->nrows * q->heads + 3) / 4 * 4;
-    rc = ensure_work(band, deltas + partial_floats(s->nslots, k->heads, q->dim));
+    const uint64_t stats = ((uint64_t)band->nrows * q->heads + 1 + 3) / 4 * 4;
+    rc = ensure_work(band, 2 * stats + partial_floats(s->nslots, k->heads, q->dim));
     if (rc)
         return rc;
     uint32_t tile_rows;
@@ -471,8 +473,9 @@ int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q, co
     a.dk = view_of(dk);
     a.dv = view_of(dv);
     a.lse = (float *)lse->dev;
-    a.delta = band->work;
-    a.partial = band->work + deltas;
+    a.stats = band->work;
+    a.nstats = stats;
+    a.partial = band->work + 2 * stats;
     a.pieces = s->pieces;
     a.splits = s->splits;
     a.npieces = s->npieces;

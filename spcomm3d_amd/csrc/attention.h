@@ -42,7 +42,10 @@ struct KeySplit {
 struct BandArgs {
     HeadsView q, k, v, o, d_o, dq, dk, dv;
     float *lse;   // [row][head]; may be null in the forward call
-    float *delta; // [row][head], sum of d_o o
+    // [row][head]: lse in base 2 (+inf for rows that see nothing), then <d_o, o>; nstats each, the
+    // last one for rows that are not there
+    float *stats;
+    uint64_t nstats;
     float *partial;
     const RowTile *tiles;
     const KeyPiece *pieces;

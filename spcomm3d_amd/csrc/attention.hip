@@ -7,6 +7,8 @@
 #include "attention_frag.h"
 #include "kernels.h"
 
+#include <type_traits>
+
 namespace spc3d {
 namespace {
 
@@ -61,12 +63,12 @@ template <typename T> __device__ __forceinline__ bool is_finite(T x) { return fa
 // leaves lane l with row l % 16, so maxima and sums of a row are over the lane's own registers and
 // two exchanges, and the probabilities are the right operand of O^T += V^T P^T where they lie.
 template <typename T, int DP, int NQ>
-__global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kernel(BandArgs a)
 {
     typedef Tile<T, DP> L;
     constexpr int NS = DP / 32, ND = DP / 16, NT = kKeyStep / 16;
-    __shared__ __align__(16) char smem[2 * kKeyStep * L::kRowBytes];
-    char *const kt = smem, *const vt = smem + kKeyStep * L::kRowBytes;
+    constexpr int kBytes = kKeyStep * L::kRowBytes;
+    __shared__ __align__(16) char tiles[2][2][kBytes]; // keys and values of this step and the next
 
     const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
     const RowTile t = a.tiles[w.tile];
@@ -92,13 +94,21 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
     const Steps st = steps_of(t.pos0, t.pos0 + (int)t.nrow - 1, ncols, a.window, a.sinks);
     const int wa = t.pos0 + wave * NQ * 16, wb = min(wa + NQ * 16, t.pos0 + (int)t.nrow) - 1;
     const float sc = a.scale * kLog2e;
+    if (dim < DP)
+        clear_tile<4 * kBytes, kThreads>(tiles[0][0], tid);
+    auto fetch = [&](int k) {
+        const int c0 = st.at(k) * (int)kKeyStep;
+        char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+        const int id = fresh(tid);
+        load_tile<T, DP, kKeyStep, kThreads>(kt, kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, id);
+        load_tile<T, DP, kKeyStep, kThreads>(vt, vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, id);
+    };
 
     f32x4 acc[ND][NQ];
     float m[NQ], sum[NQ];
-    TileCopy<T, DP, kKeyStep, kThreads> ck, cv;
     // The second pass, if any, is for values that are not finite: 0 x inf would reach rows that do
     // not see them, so steps with hidden pairs take those values one by one.
-    for (int careful = 0; careful < 2; ++careful) {
+    auto pass = [&](auto careful) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             m[n] = kNegInf;
@@ -107,22 +117,17 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
             for (int d = 0; d < ND; ++d)
                 acc[d][n] = f32x4{0, 0, 0, 0};
         }
-        if (st.count > 0) {
-            const int c0 = st.at(0) * (int)kKeyStep;
-            ck.load(kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, tid);
-            cv.load(vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, tid);
-        }
+        __syncthreads(); // the tiles are cleared, or read for the last time
+        if (st.count > 0)
+            fetch(0);
         for (int k = 0; k < st.count; ++k) {
             const int c0 = st.at(k) * (int)kKeyStep;
+            char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+            const int lane = fresh(tid & 63);
+            loads_done();
             __syncthreads();
-            ck.store(kt, tid);
-            cv.store(vt, tid);
-            __syncthreads();
-            if (k + 1 < st.count) {
-                const int c1 = st.at(k + 1) * (int)kKeyStep;
-                ck.load(kp + c1 * a.k.stride, a.k.stride, ncols - c1, dim, tid);
-                cv.load(vp + c1 * a.v.stride, a.v.stride, ncols - c1, dim, tid);
-            }
+            if (k + 1 < st.count)
+                fetch(k + 1);
             const int c9 = c0 + (int)kKeyStep - 1;
             if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
                 continue; // nothing here is seen by this wavefront's rows
@@ -152,18 +157,35 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
                             if (!sees(pos[n], c0 + 16 * i + 4 * g + j, a.window, a.sinks))
                                 sv[i][n][j] = kNegInf;
             }
+            float top[NQ];
+            bool grown = false;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                float top = sv[0][n][0];
+                top[n] = sv[0][n][0];
 #pragma unroll
                 for (int i = 0; i < NT; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        top = fmaxf(top, sv[i][n][j]);
-                top = fmaxf(m[n], column_max(top) * sc);
-                const float base = top == kNegInf ? 0.0f : top; // nothing seen yet: exp2(-inf - 0) = 0
-                const float down = __builtin_amdgcn_exp2f(m[n] - base), less = base - WeightShift<T>::value;
-                m[n] = top;
+                        top[n] = fmaxf(top[n], sv[i][n][j]);
+                top[n] = column_max(top[n]) * sc;
+                grown |= top[n] > m[n] + kSlack;
+            }
+            if (__any(grown)) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    const float to = fmaxf(m[n], top[n]);
+                    const float down = __builtin_amdgcn_exp2f(m[n] - (to == kNegInf ? 0.0f : to));
+                    m[n] = to;
+                    sum[n] *= down;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        acc[d][n] *= down;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                // nothing seen yet: exp2(-inf - 0) = 0
+                const float less = (m[n] == kNegInf ? 0.0f : m[n]) - WeightShift<T>::value;
                 float add = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NT; ++i)
@@ -173,25 +195,22 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
                         sv[i][n][j] = p;
                         add += p;
                     }
-                sum[n] = sum[n] * down + add;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    acc[d][n] *= down;
+                sum[n] += add;
             }
-            const bool one_by_one = careful && !whole;
+            const bool one_by_one = careful.value && !whole;
 #pragma unroll
             for (int u = 0; u < NT / 2; ++u) {
                 Frag<T> pf[NQ];
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
-                    pf[n] = join<T>(sv[2 * u][n], sv[2 * u + 1][n]);
+                    pf[n] = join<T>(rounded<T>(sv[2 * u][n]), rounded<T>(sv[2 * u + 1][n]));
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> f = L::columns(vt, 32 * u, d, lane);
-                    if (one_by_one) {
+                    if constexpr (careful.value) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            if (!is_finite(f[j]))
+                            if (one_by_one && !is_finite(f[j]))
                                 f[j] = (T)0.0f;
                     }
 #pragma unroll
@@ -231,9 +250,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
                     bad |= mine && !is_finite(acc[d][n][j]);
             }
         }
-        if (careful || !__syncthreads_or(bad))
-            break;
-    }
+        return bad;
+    };
+    if (__syncthreads_or(pass(std::false_type())))
+        pass(std::true_type());
     T *const op = (T *)a.o.p + t.row0 * a.o.stride + w.head * dim;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -255,12 +275,12 @@ __global__ __launch_bounds__(kThreads, 2) void attend_kernel(BandArgs a)
 // again: seven products instead of five, but every sum is one workgroup's, in a fixed order,
 // without atomics or a panel of partial dQ.
 template <typename T, int DP, int NQ>
-__global__ __launch_bounds__(kThreads, 1) void attend_dq_kernel(BandArgs a)
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_kernel(BandArgs a)
 {
     typedef Tile<T, DP> L;
     constexpr int NS = DP / 32, ND = DP / 16, NT = kKeyStep / 16;
-    __shared__ __align__(16) char smem[2 * kKeyStep * L::kRowBytes];
-    char *const kt = smem, *const vt = smem + kKeyStep * L::kRowBytes;
+    constexpr int kBytes = kKeyStep * L::kRowBytes;
+    __shared__ __align__(16) char tiles[2][2][kBytes]; // keys and values of this step and the next
 
     const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
     const RowTile t = a.tiles[w.tile];
@@ -301,14 +321,22 @@ __global__ __launch_bounds__(kThreads, 1) void attend_dq_kernel(BandArgs a)
     const Steps st = steps_of(t.pos0, t.pos0 + (int)t.nrow - 1, ncols, a.window, a.sinks);
     const int wa = t.pos0 + wave * NQ * 16, wb = min(wa + NQ * 16, t.pos0 + (int)t.nrow) - 1;
     const float sc = a.scale * kLog2e;
+    if (dim < DP)
+        clear_tile<4 * kBytes, kThreads>(tiles[0][0], tid);
+    auto fetch = [&](int k) {
+        const int c0 = st.at(k) * (int)kKeyStep;
+        char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+        const int id = fresh(tid);
+        load_tile<T, DP, kKeyStep, kThreads>(kt, kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, id);
+        load_tile<T, DP, kKeyStep, kThreads>(vt, vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, id);
+    };
 
     f32x4 acc[ND][NQ];
-    TileCopy<T, DP, kKeyStep, kThreads> ck, cv;
     float weighed[NQ]; // sum of P dP: <dO, o> again, without the rounding of o
     // Rows that see few columns take it before they use it: their dS is a small difference, and
     // the rounding of o in <dO, o> would show (dQ of 300 rows in bfloat16: 1.72 times the error of
     // one rounding, 1.47 so; further down the sequence it is lost among the columns).
-    for (int last = st.count > kFewSteps; last < 2; ++last) {
+    auto pass = [&](auto last) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             weighed[n] = 0.0f;
@@ -316,75 +344,83 @@ __global__ __launch_bounds__(kThreads, 1) void attend_dq_kernel(BandArgs a)
             for (int d = 0; d < ND; ++d)
                 acc[d][n] = f32x4{0, 0, 0, 0};
         }
-        if (st.count > 0) {
-            const int c0 = st.at(0) * (int)kKeyStep;
-            ck.load(kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, tid);
-            cv.load(vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, tid);
-        }
+        __syncthreads(); // the tiles are cleared, or read for the last time
+        if (st.count > 0)
+            fetch(0);
         for (int k = 0; k < st.count; ++k) {
             const int c0 = st.at(k) * (int)kKeyStep;
+            char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+            const int lane = fresh(tid & 63);
+            loads_done();
             __syncthreads();
-            ck.store(kt, tid);
-            cv.store(vt, tid);
-            __syncthreads();
-            if (k + 1 < st.count) {
-                const int c1 = st.at(k + 1) * (int)kKeyStep;
-                ck.load(kp + c1 * a.k.stride, a.k.stride, ncols - c1, dim, tid);
-                cv.load(vp + c1 * a.v.stride, a.v.stride, ncols - c1, dim, tid);
-            }
+            if (k + 1 < st.count)
+                fetch(k + 1);
             const int c9 = c0 + (int)kKeyStep - 1;
             if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
                 continue;
             const bool whole = c9 <= wa && (wb - c0 < a.window || c9 < a.sinks);
 #pragma unroll
             for (int u = 0; u < NT / 2; ++u) {
-                f32x4 sv[2][NQ], dp[2][NQ];
+                HalfFrag<T> ds[2][NQ];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
+                    f32x4 sv[NQ], dp[NQ];
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
-                        sv[i][n] = dp[i][n] = f32x4{0, 0, 0, 0};
+                        sv[n] = dp[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int s = 0; s < NS; ++s) {
                         const Frag<T> f = L::rows(kt, 32 * u + 16 * i, s, lane);
                         const Frag<T> h = L::rows(vt, 32 * u + 16 * i, s, lane);
 #pragma unroll
                         for (int n = 0; n < NQ; ++n) {
-                            sv[i][n] = mma(f, qf[n][s], sv[i][n]);
-                            dp[i][n] = mma(h, gf[n][s], dp[i][n]);
+                            sv[n] = mma(f, qf[n][s], sv[n]);
+                            dp[n] = mma(h, gf[n][s], dp[n]);
                         }
                     }
+                    if (!whole) {
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n)
+                        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (!sees(pos[n], c0 + 32 * u + 16 * i + 4 * g + j, a.window, a.sinks)) {
+                                    sv[n][j] = kNegInf;
+                                    dp[n][j] = 0.0f;
+                                }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i][n][j], sc, -lse[n]));
-                            float y = dp[i][n][j];
-                            if (!whole && !sees(pos[n], c0 + 32 * u + 16 * i + 4 * g + j, a.window, a.sinks))
-                                p = y = 0.0f;
-                            weighed[n] = __builtin_fmaf(p, y, weighed[n]);
-                            sv[i][n][j] = p * (y - delta[n]);
+                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[n][j], sc, -lse[n]));
+                            weighed[n] = __builtin_fmaf(p, dp[n][j], weighed[n]);
+                            sv[n][j] = p * (dp[n][j] - delta[n]);
                         }
+                        ds[i][n] = rounded<T>(sv[n]);
+                    }
                 }
-                if (!last)
-                    continue;
-                Frag<T> df[NQ];
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-                    df[n] = join<T>(sv[0][n], sv[1][n]);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const Frag<T> f = L::columns(kt, 32 * u, d, lane);
+                if constexpr (last.value) {
+                    Frag<T> df[NQ];
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
-                        acc[d][n] = mma(f, df[n], acc[d][n]);
+                        df[n] = join<T>(ds[0][n], ds[1][n]);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const Frag<T> f = L::columns(kt, 32 * u, d, lane);
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n)
+                            acc[d][n] = mma(f, df[n], acc[d][n]);
+                    }
                 }
             }
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
             delta[n] = column_sum(weighed[n]);
-    }
+    };
+    if (st.count <= kFewSteps)
+        pass(std::false_type());
+    pass(std::true_type());
     T *const dqp = (T *)a.dq.p + t.row0 * a.dq.stride + w.head * dim;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -395,24 +431,31 @@ __global__ __launch_bounds__(kThreads, 1) void attend_dq_kernel(BandArgs a)
         for (int d = 0; d < ND; ++d)
             if (16 * d + 4 * g < dim)
                 store_half<T>(dqp + r * a.dq.stride + 16 * d + 4 * g, acc[d][n] * a.scale);
-        if (g == 0)
-            a.delta[(uint64_t)(t.row0 + r) * a.heads + w.head] = delta[n];
+        if (g == 0) {
+            const uint64_t at = (uint64_t)(t.row0 + r) * a.heads + w.head;
+            a.stats[at] = lse[n];
+            a.stats[a.nstats + at] = delta[n];
+        }
+    }
+    if (blockIdx.x == 0 && tid == 0) { // what rows past a tile's end read
+        a.stats[a.nstats - 1] = -kNegInf;
+        a.stats[2 * a.nstats - 1] = 0.0f;
     }
 }
 
 // Each wavefront owns 32 columns of the tile's 128, whose keys and values stay in its registers;
-// rows (of every head that shares them) come through LDS 32 at a time.  S = Q K^T leaves a lane
+// rows (of every head that shares them) come through LDS 64 at a time.  S = Q K^T leaves a lane
 // with one column and the rows 4 g + i, 16 + 4 g + i, which is the left operand of dV += P^T dO and
 // dK += dS^T Q as it lies.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, 1) void attend_dkv_kernel(BandArgs a)
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_kernel(BandArgs a)
 {
     typedef Tile<T, DP> L;
-    constexpr int NS = DP / 32, ND = DP / 16, NK = 2, ROWS = 32;
-    constexpr float kUp = WeightShift<T>::value ? 32768.0f : 1.0f;
-    __shared__ __align__(16) char smem[2 * ROWS * L::kRowBytes];
-    __shared__ __align__(16) float row_lse[ROWS], row_delta[ROWS];
-    char *const qt = smem, *const gt = smem + ROWS * L::kRowBytes;
+    constexpr int NS = DP / 32, ND = DP / 16, NK = 2, ROWS = 64;
+    constexpr float kUp = sizeof(T) == 2 && WeightShift<T>::value != 0 ? 32768.0f : 1.0f; // weights are at most 1 here
+    constexpr int kBytes = ROWS * L::kRowBytes;
+    __shared__ __align__(16) char tiles[2][2][kBytes]; // Q and dO of this step and the next
+    __shared__ __align__(16) float stats[2][2 * ROWS]; // lse and <dO, o> of their rows
 
     const uint32_t group = a.heads / a.kv_heads;
     const Work w = work_of(blockIdx.x, a.npieces, a.kv_heads, a.kv_heads);
@@ -440,38 +483,39 @@ __global__ __launch_bounds__(kThreads, 1) void attend_dkv_kernel(BandArgs a)
         for (int d = 0; d < ND; ++d)
             dk[n][d] = dv[n][d] = f32x4{0, 0, 0, 0};
     }
-    const int ca = t.col0 + wave * NK * 16, cb = ca + NK * 16 - 1;
+    const int wave_first = __builtin_amdgcn_readfirstlane(wave * NK * 16);
+    const int ca = t.col0 + wave_first, cb = ca + NK * 16 - 1;
     const float sc = a.scale * kLog2e;
     const int per = (nrow + ROWS - 1) / ROWS, count = per * (int)group;
 
-    TileCopy<T, DP, ROWS, kThreads> cq, cg;
-    float next_lse = 0.0f, next_delta = 0.0f;
+    if (dim < DP)
+        clear_tile<4 * kBytes, kThreads>(tiles[0][0], tid);
     auto fetch = [&](int k) {
+        char *const qt = tiles[k & 1][0], *const gt = tiles[k & 1][1];
         const uint32_t head = w.head * group + k / per;
         const int r0 = (k % per) * ROWS;
         const uint64_t row = t.row0 + r0;
-        cq.load((const T *)a.q.p + row * a.q.stride + head * dim, a.q.stride, nrow - r0, dim, tid);
-        cg.load((const T *)a.d_o.p + row * a.d_o.stride + head * dim, a.d_o.stride, nrow - r0, dim, tid);
-        if (tid < ROWS) {
-            next_lse = -kNegInf; // rows past the end and rows that see nothing weigh nothing
-            next_delta = 0.0f;
-            if (r0 + tid < nrow) {
-                const float x = a.lse[(row + tid) * a.heads + head] * kLog2e;
-                next_lse = x == kNegInf ? -kNegInf : x;
-                next_delta = a.delta[(row + tid) * a.heads + head];
-            }
+        const int id = fresh(tid);
+        load_tile<T, DP, ROWS, kThreads>(qt, (const T *)a.q.p + row * a.q.stride + head * dim, a.q.stride, nrow - r0,
+                                         dim, id);
+        load_tile<T, DP, ROWS, kThreads>(gt, (const T *)a.d_o.p + row * a.d_o.stride + head * dim, a.d_o.stride,
+                                         nrow - r0, dim, id);
+        const int which = __builtin_amdgcn_readfirstlane(id >> 6);
+        if (which < 2) { // rows past the end weigh nothing
+            const int r = id & 63;
+            const uint64_t at = r0 + r < nrow ? (row + r) * a.heads + head : a.nstats - 1;
+            __builtin_amdgcn_global_load_lds((global_void *)(a.stats + which * a.nstats + at),
+                                             (lds_void *)(stats[k & 1] + which * ROWS), 4, 0, 0);
         }
     };
+    __syncthreads();
     if (count > 0)
         fetch(0);
     for (int k = 0; k < count; ++k) {
-        __syncthreads();
-        cq.store(qt, tid);
-        cg.store(gt, tid);
-        if (tid < ROWS) {
-            row_lse[tid] = next_lse;
-            row_delta[tid] = next_delta;
-        }
+        char *const qt = tiles[k & 1][0], *const gt = tiles[k & 1][1];
+        const float *const stat = stats[k & 1];
+        const int lane = fresh(tid & 63);
+        loads_done();
         __syncthreads();
         if (k + 1 < count)
             fetch(k + 1);
@@ -480,51 +524,64 @@ __global__ __launch_bounds__(kThreads, 1) void attend_dkv_kernel(BandArgs a)
             continue;
         const bool whole = pa >= cb && (pb - ca < a.window || cb < a.sinks);
 
-        f32x4 sv[2][NK], dp[2][NK];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int u = 0; u < ROWS / 32; ++u) {
+            HalfFrag<T> ps[2][NK], ds[2][NK];
 #pragma unroll
-            for (int n = 0; n < NK; ++n)
-                sv[i][n] = dp[i][n] = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < 2; ++i) {
+                f32x4 sv[NK], dp[NK];
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const Frag<T> f = L::rows(qt, 16 * i, s, lane);
-                const Frag<T> h = L::rows(gt, 16 * i, s, lane);
+                for (int n = 0; n < NK; ++n)
+                    sv[n] = dp[n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const Frag<T> f = L::rows(qt, 32 * u + 16 * i, s, lane);
+                    const Frag<T> h = L::rows(gt, 32 * u + 16 * i, s, lane);
+#pragma unroll
+                    for (int n = 0; n < NK; ++n) {
+                        sv[n] = mma(f, kf[n][s], sv[n]);
+                        dp[n] = mma(h, vf[n][s], dp[n]);
+                    }
+                }
+                const f32x4 lse = *reinterpret_cast<const f32x4 *>(stat + 32 * u + 16 * i + 4 * g);
+                const f32x4 delta = *reinterpret_cast<const f32x4 *>(stat + ROWS + 32 * u + 16 * i + 4 * g);
+                if (!whole) {
+#pragma unroll
+                    for (int n = 0; n < NK; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (!sees(pa + 32 * u + 16 * i + 4 * g + j, col[n], a.window, a.sinks)) {
+                                sv[n][j] = kNegInf;
+                                dp[n][j] = 0.0f;
+                            }
+                }
 #pragma unroll
                 for (int n = 0; n < NK; ++n) {
-                    sv[i][n] = mma(f, kf[n][s], sv[i][n]);
-                    dp[i][n] = mma(h, vf[n][s], dp[i][n]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[n][j], sc, -lse[j]));
+                        sv[n][j] = p * kUp;
+                        dp[n][j] = p * (dp[n][j] - delta[j]);
+                    }
+                    ps[i][n] = rounded<T>(sv[n]);
+                    ds[i][n] = rounded<T>(dp[n]);
                 }
             }
-            const f32x4 lse = *reinterpret_cast<const f32x4 *>(row_lse + 16 * i + 4 * g);
-            const f32x4 delta = *reinterpret_cast<const f32x4 *>(row_delta + 16 * i + 4 * g);
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i][n][j], sc, -lse[j]));
-                    float ds = p * (dp[i][n][j] - delta[j]);
-                    p *= kUp;
-                    if (!whole && !sees(pa + 16 * i + 4 * g + j, col[n], a.window, a.sinks))
-                        p = ds = 0.0f;
-                    sv[i][n][j] = p;
-                    dp[i][n][j] = ds;
-                }
-        }
-        Frag<T> pf[NK], df[NK];
-#pragma unroll
-        for (int n = 0; n < NK; ++n) {
-            pf[n] = join<T>(sv[0][n], sv[1][n]);
-            df[n] = join<T>(dp[0][n], dp[1][n]);
-        }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            const Frag<T> f = L::columns(gt, 0, d, lane);
-            const Frag<T> h = L::columns(qt, 0, d, lane);
+            Frag<T> pf[NK], df[NK];
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
-                dv[n][d] = mma(pf[n], f, dv[n][d]);
-                dk[n][d] = mma(df[n], h, dk[n][d]);
+                pf[n] = join<T>(ps[0][n], ps[1][n]);
+                df[n] = join<T>(ds[0][n], ds[1][n]);
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const Frag<T> f = L::columns(gt, 32 * u, d, lane);
+                const Frag<T> h = L::columns(qt, 32 * u, d, lane);
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    dv[n][d] = mma(pf[n], f, dv[n][d]);
+                    dk[n][d] = mma(df[n], h, dk[n][d]);
+                }
             }
         }
     }

@@ -60,18 +60,19 @@ template <typename T> __device__ __forceinline__ Frag<T> zero_frag()
     return f;
 }
 
-// The rows of two results as the k of the next product, rounded once to T.
-template <typename T> __device__ __forceinline__ Frag<T> join(f32x4 lo, f32x4 hi)
+// Four results rounded to T; two such are the k of the next product.
+template <typename T> __device__ __forceinline__ HalfFrag<T> rounded(f32x4 x)
 {
-    Frag<T> f;
+    HalfFrag<T> f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[i] = (T)lo[i];
-        f[4 + i] = (T)hi[i];
-    }
+    for (int i = 0; i < 4; ++i)
+        f[i] = (T)x[i];
     return f;
 }
-
+template <typename T> __device__ __forceinline__ Frag<T> join(HalfFrag<T> lo, HalfFrag<T> hi)
+{
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 // Eight elements of a row in global memory, 16-byte aligned.
 template <typename T> __device__ __forceinline__ Frag<T> load_frag(const T *p)
 {
@@ -84,11 +85,7 @@ template <typename T> __device__ __forceinline__ Frag<T> load_frag(const T *p)
 }
 template <typename T> __device__ __forceinline__ void store_half(T *p, f32x4 v)
 {
-    HalfFrag<T> h;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        h[i] = (T)v[i];
-    *reinterpret_cast<HalfFrag<T> *>(p) = h;
+    *reinterpret_cast<HalfFrag<T> *>(p) = rounded<T>(v);
 }
 
 // A tile of rows in LDS, DP elements of each, cut into chunks of 16 bytes; chunk c of row r lies
@@ -148,34 +145,44 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// ROWS rows of a panel on their way to an LDS tile through the registers of THREADS threads.  Rows
-// from nrow on repeat row nrow - 1 (nrow >= 1; their scores are masked), elements from dim on are 0.
-template <typename T, int DP, int ROWS, int THREADS> struct TileCopy {
-    typedef Tile<T, DP> L;
-    static constexpr int kAll = ROWS * L::kUsed, kEach = (kAll + THREADS - 1) / THREADS;
-    u32x4 reg[kEach];
+// ROWS rows of a panel straight into an LDS tile, without registers between: a wavefront's load
+// fills 1 KiB in lane order, so each lane asks for the chunk whose place is its own.  Rows from nrow on
+// repeat row nrow - 1 (nrow >= 1; their scores are masked); chunks from dim on are left alone
+// (clear_tile).  The loads are under way when this returns: loads_done(), then a barrier.
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
 
-    __device__ __forceinline__ void load(const T *src, uint64_t stride, int nrow, int dim, int tid)
-    {
+template <typename T, int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void load_tile(char *tile, const T *src, uint64_t stride, int nrow, int dim, int tid)
+{
+    typedef Tile<T, DP> L;
+    constexpr int kLoads = ROWS * L::kChunks / THREADS, kStep = THREADS / L::kChunks; // rows of a load
+    static_assert(ROWS % kStep == 0, "whole loads");
+    const int first = __builtin_amdgcn_readfirstlane(tid & ~63), r0 = tid / L::kChunks;
+    const uint32_t row_bytes = (uint32_t)stride * sizeof(T); // rows are at most 2^22 elements long
+    auto load = [&](int i, uint32_t r, const char *from) {
+        const int c = (tid % L::kChunks) ^ L::mix(r0 + i * kStep);
+        if (c * L::kVec < dim)
+            __builtin_amdgcn_global_load_lds((global_void *)(from + (r * row_bytes + c * 16)),
+                                             (lds_void *)(tile + (i * THREADS + first) * 16), 16, 0, 0);
+    };
+    if (nrow >= ROWS) { // one offset for every load, from a base of its own
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int id = i * THREADS + tid, c = id % L::kUsed, r = id / L::kUsed;
-            const int rr = r < nrow ? r : nrow - 1;
-            reg[i] = u32x4{0, 0, 0, 0};
-            if (c * L::kVec < dim && (kAll % THREADS == 0 || id < kAll))
-                reg[i] = *reinterpret_cast<const u32x4 *>(src + rr * stride + c * L::kVec);
-        }
-    }
-    __device__ __forceinline__ void store(char *tile, int tid) const
-    {
+        for (int i = 0; i < kLoads; ++i)
+            load(i, r0, (const char *)src + (uint64_t)(i * kStep) * row_bytes);
+    } else {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int id = i * THREADS + tid, c = id % L::kUsed, r = id / L::kUsed;
-            if (kAll % THREADS == 0 || id < kAll)
-                *reinterpret_cast<u32x4 *>(tile + L::at(r, c)) = reg[i];
-        }
+        for (int i = 0; i < kLoads; ++i)
+            load(i, min(r0 + i * kStep, nrow - 1), (const char *)src);
     }
-};
+}
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); } // vmcnt(0)
+
+template <int BYTES, int THREADS> __device__ __forceinline__ void clear_tile(char *tile, int tid)
+{
+    for (int i = tid * 16; i < BYTES; i += THREADS * 16)
+        *reinterpret_cast<u32x4 *>(tile + i) = u32x4{0, 0, 0, 0};
+}
 
 // e4m3, to nearest even; what is too large for it becomes the largest (448), NaN stays NaN.
 constexpr float kF8Most = 448.0f;
@@ -186,24 +193,41 @@ __device__ __forceinline__ uint8_t to_f8(float x)
     return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
 }
 
-// Weights are at most 1, and half keeps its bits only down to 2^-14: in half they are 2^15 times
-// themselves on their way through the matrix instructions (the sums that divide them as well).
+// Weights are exp2(score - base) with a base that follows the running maximum only when a score is
+// more than kSlack above it: most steps then leave the sums so far as they are.  Half keeps its bits only down to 2^-14, so
+// weights are 2^value times themselves on their way through the matrix instructions (and so are
+// the sums that divide them): 2^(8 + 7) at most.
+constexpr float kSlack = 7.0f;
 template <typename T> struct WeightShift { static constexpr float value = 0.0f; };
-template <> struct WeightShift<f16_t> { static constexpr float value = 15.0f; };
+template <> struct WeightShift<f16_t> { static constexpr float value = 8.0f; };
+
+// The same number, of which the compiler knows nothing more: addresses made from it inside a loop
+// are made there again instead of being kept in registers that the accumulators need.
+__device__ __forceinline__ int fresh(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
 
-// Over the four lanes that hold the same column of a result.
+// Over the four lanes that hold the same column of a result: each exchange leaves one number of
+// either half in every lane.
+template <typename F> __device__ __forceinline__ float over_column(float x, F f)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float column_max(float x)
 {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    return over_column(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float column_sum(float x)
 {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    return over_column(x, [](float a, float b) { return a + b; });
 }
 
 } // namespace spc3d

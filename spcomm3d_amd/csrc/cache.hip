@@ -476,7 +476,7 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
                 Frag<T> pf[NC];
 #pragma unroll
                 for (int n = 0; n < NC; ++n)
-                    pf[n] = join<T>(sv[2 * u][n], sv[2 * u + 1][n]);
+                    pf[n] = join<T>(rounded<T>(sv[2 * u][n]), rounded<T>(sv[2 * u + 1][n]));
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> f;
