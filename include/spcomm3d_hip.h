@@ -582,7 +582,7 @@ typedef struct {
 } spc3d_heads;
 typedef struct spc3d_band spc3d_band;
 /* The pattern of a call: its sequences cut into tiles, on the device.  rows[] and cols[] (nseq
- * each, host memory) are copied.  The first spc3d_attend_grad with a number of kv heads lays out
+ * each, host memory) are copied.  The first spc3d_attend_grad with a number of heads lays out
  * its pieces of columns and its workspace, kept with the band (so not while recording). */
 SPC3D_API int spc3d_band_create(spc3d_ctx *ctx, uint32_t nseq, const uint32_t *rows,
                       const uint32_t *cols, uint32_t window, uint32_t sinks, spc3d_band **out);

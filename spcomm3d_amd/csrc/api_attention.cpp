@@ -7,12 +7,13 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <functional>
 
 namespace {
 
-// The pieces that spc3d_attend_grad's column kernel works on, for one number of kv heads.
+// The pieces that spc3d_attend_grad's column kernel works on, for one number of heads.
 struct KeySchedule {
-    uint32_t kv_heads = 0, npieces = 0, nsplits = 0, nslots = 0;
+    uint32_t kv_heads = 0, group = 0, npieces = 0, nsplits = 0, nslots = 0;
     KeyPiece *pieces = nullptr;
     KeySplit *splits = nullptr;
 };
@@ -109,67 +110,122 @@ std::vector<RowTile> row_tiles(const spc3d_band *b, uint32_t size)
     return tiles;
 }
 
-// Tiles of kKeyTile columns, each with the rows that see one of them.  A tile that far more rows
-// see than others (the first columns, or any without a window) is cut into pieces of rows, about
-// four for each CU over all kv heads and none under 128 rows; the pieces' sums are joined.
-void key_pieces(const spc3d_band *b, uint32_t kv_heads, std::vector<KeyPiece> &pieces,
+// How many units of work the longest of `slots` workers gets when each in turn takes the next of
+// `costs` (descending).
+uint64_t makespan(const std::vector<uint64_t> &costs, size_t slots)
+{
+    if (costs.size() <= slots)
+        return costs.empty() ? 0 : costs.front();
+    std::vector<uint64_t> heap(slots, 0); // the least loaded on top
+    for (uint64_t c : costs) {
+        std::pop_heap(heap.begin(), heap.end(), std::greater<uint64_t>());
+        heap.back() += c;
+        std::push_heap(heap.begin(), heap.end(), std::greater<uint64_t>());
+    }
+    return *std::max_element(heap.begin(), heap.end());
+}
+
+// Tiles of kKeyTile columns, each with the rows that see one of them, cut into pieces of steps
+// where that ends sooner.  Rows that see a tile for its sinks alone are pieces of their own.
+// The choice goes by what the parts of a call cost on an MI355X, in steps of kRowStep rows (7 us with
+// two workgroups on a CU, heads of 128 in 16 bits): half a step to begin and end a piece, two more
+// to write its partial sums, half a step of the whole GPU for the launch that joins them and 1/512
+// for each piece in it.
+void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, std::vector<KeyPiece> &pieces,
                 std::vector<KeySplit> &splits, uint32_t *nslots)
 {
     std::vector<KeyPiece> tiles;
-    uint64_t total = 0;
     uint32_t row0 = 0, key0 = 0;
+    uint64_t longest = 1;
+    auto add = [&](KeyPiece t, int64_t lo, int64_t hi, int64_t off) { // rows lo .. hi of the sequence
+        t.row0 = row0 + (uint32_t)lo;
+        t.nrow = (uint32_t)std::max<int64_t>(0, hi - lo);
+        t.pos0 = (int32_t)(lo + off);
+        t.nsteps = (t.nrow + kRowStep - 1) / kRowStep * group;
+        t.slot = kNoSlot;
+        longest = std::max<uint64_t>(longest, t.nsteps);
+        tiles.push_back(t);
+    };
     for (size_t s = 0; s < b->rows.size(); ++s) {
         const int64_t n = b->rows[s], m = b->cols[s], off = m - n;
         for (int64_t c = 0; c < m; c += kKeyTile) {
             KeyPiece t = {};
             t.nkey = (uint32_t)std::min<int64_t>(kKeyTile, m - c);
-            const int64_t lo = std::max<int64_t>(0, c - off);
-            int64_t hi = n;
-            if (c >= b->sinks)
-                hi = std::min(n, c + t.nkey - 1 + b->window - off);
             t.key0 = key0 + (uint32_t)c;
-            t.row0 = row0 + (uint32_t)std::min(lo, n);
-            t.nrow = (uint32_t)std::max<int64_t>(0, hi - lo);
-            t.pos0 = (int32_t)(lo + off);
             t.col0 = (int32_t)c;
-            t.slot = kNoSlot;
-            tiles.push_back(t);
-            total += t.nrow;
+            const int64_t lo = std::min(n, std::max<int64_t>(0, c - off));
+            const int64_t near = std::min(n, std::max(lo, c + t.nkey - 1 + b->window - off)); // the window's rows
+            const bool spread = c < b->sinks && b->sinks - c <= (int64_t)kSpread && near < n;
+            add(t, lo, c < b->sinks && !spread ? n : near, off);
+            if (spread) {
+                t.spread = 1;
+                add(t, near, n, off);
+            }
         }
         row0 += (uint32_t)n;
         key0 += (uint32_t)m;
     }
-    const uint64_t want = std::max<uint64_t>(1, 4ull * b->ctx->cu_count / kv_heads);
-    const uint32_t most = (uint32_t)((std::max<uint64_t>(128, (total + want - 1) / want) + 63) / 64 * 64);
-    uint32_t slots = 0;
-    for (const KeyPiece &t : tiles) {
-        const uint32_t count = (t.nrow + most - 1) / most;
-        if (count <= 1) {
-            pieces.push_back(t);
-            continue;
+    // the longest piece allowed, by trial
+    const size_t slots = std::max<size_t>(1, 2 * (size_t)b->ctx->cu_count / kv_heads);
+    auto count_of = [&](const KeyPiece &t, uint64_t most) {
+        const uint64_t all = t.spread ? (t.nsteps + 1) / 2 : t.nsteps; // a spread step costs half of one
+        return (uint32_t)std::max<uint64_t>(1, (all + most - 1) / most);
+    };
+    uint64_t best = longest, best_cost = UINT64_MAX;
+    std::vector<uint64_t> costs;
+    for (uint64_t most = longest, before = 0; most >= 1; most = most * 3 / 4) {
+        if (most == before)
+            break;
+        before = most;
+        costs.clear();
+        uint64_t joined = 0;
+        for (size_t i = 0; i < tiles.size(); ++i) {
+            const KeyPiece &t = tiles[i];
+            const uint32_t count = count_of(t, most);
+            const bool split = count > 1 || t.spread || (i + 1 < tiles.size() && tiles[i + 1].spread);
+            const uint64_t each = 512ull * t.nsteps / count / (t.spread ? 2 : 1);
+            for (uint32_t k = 0; k < count; ++k)
+                costs.push_back(each + 256 + (split ? 1024 : 0));
+            joined += split ? count : 0;
         }
-        const uint32_t each = ((t.nrow + count - 1) / count + 63) / 64 * 64;
-        KeySplit sp = {t.key0, t.nkey, slots, 0};
-        for (uint32_t r = 0; r < t.nrow; r += each) {
-            KeyPiece p = t;
-            p.row0 += r;
-            p.pos0 += (int32_t)r;
-            p.nrow = std::min(each, t.nrow - r);
-            p.slot = slots++;
-            ++sp.count;
-            pieces.push_back(p);
+        if (costs.size() > 16 * slots && best_cost != UINT64_MAX)
+            break;
+        std::sort(costs.begin(), costs.end(), std::greater<uint64_t>());
+        const uint64_t cost = makespan(costs, slots) + (joined ? 256 + joined * kv_heads : 0);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = most;
         }
-        splits.push_back(sp);
     }
-    std::stable_sort(pieces.begin(), pieces.end(),
-                     [](const KeyPiece &x, const KeyPiece &y) { return x.nrow > y.nrow; });
-    *nslots = slots;
+    uint32_t next = 0;
+    std::vector<std::pair<uint64_t, KeyPiece>> all;
+    for (size_t i = 0; i < tiles.size(); ++i) {
+        const KeyPiece &t = tiles[i];
+        const uint32_t count = count_of(t, best);
+        const bool lone = count == 1 && !t.spread && !(i + 1 < tiles.size() && tiles[i + 1].spread);
+        if (!lone && !t.spread)
+            splits.push_back(KeySplit{t.key0, t.nkey, next, count, 0, {}});
+        if (t.spread)
+            splits.back().spread = count;
+        for (uint32_t k = 0; k < count; ++k) {
+            KeyPiece p = t;
+            p.step0 = (uint32_t)((uint64_t)t.nsteps * k / count);
+            p.nsteps = (uint32_t)((uint64_t)t.nsteps * (k + 1) / count) - p.step0;
+            if (!lone)
+                p.slot = next++;
+            all.push_back({t.spread ? p.nsteps / 2 : p.nsteps, p});
+        }
+    }
+    std::stable_sort(all.begin(), all.end(), [](const auto &x, const auto &y) { return x.first > y.first; });
+    for (const auto &p : all)
+        pieces.push_back(p.second);
+    *nslots = next;
 }
 
-int schedule_of(spc3d_band *b, uint32_t kv_heads, KeySchedule **out)
+int schedule_of(spc3d_band *b, uint32_t kv_heads, uint32_t group, KeySchedule **out)
 {
     for (KeySchedule &s : b->schedules)
-        if (s.kv_heads == kv_heads) {
+        if (s.kv_heads == kv_heads && s.group == group) {
             *out = &s;
             return SPC3D_OK;
         }
@@ -177,10 +233,11 @@ int schedule_of(spc3d_band *b, uint32_t kv_heads, KeySchedule **out)
         return rc;
     KeySchedule s;
     s.kv_heads = kv_heads;
+    s.group = group;
     std::vector<KeyPiece> pieces;
     std::vector<KeySplit> splits;
     try {
-        key_pieces(b, kv_heads, pieces, splits, &s.nslots);
+        key_pieces(b, kv_heads, group, pieces, splits, &s.nslots);
         b->schedules.reserve(b->schedules.size() + 1);
     } catch (const std::bad_alloc &) {
         return fail(SPC3D_ERR_ALLOC, "host allocation failed");
@@ -456,7 +513,7 @@ int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q, co
     if (rc)
         return rc;
     KeySchedule *s = nullptr;
-    rc = schedule_of(band, k->heads, &s);
+    rc = schedule_of(band, k->heads, q->heads / k->heads, &s);
     if (rc)
         return rc;
     if ((uint64_t)s->npieces * k->heads > INT_MAX || s->nsplits > INT_MAX || k->heads > 65535)

@@ -26,17 +26,23 @@ struct RowTile {
 };
 
 // A piece of a tile of columns: columns col0 .. col0 + nkey of their sequence, rows key0 .. of the
-// packed keys, and the rows row0 .. row0 + nrow (from position pos0 on) that this piece goes over.
+// packed keys.  The rows row0 .. row0 + nrow (from position pos0 on) of every head that shares the
+// columns see some of them; in steps of kRowStep rows, head after head, this piece takes the steps
+// step0 .. step0 + nsteps.
 // slot: where its partial sums go, or kNoSlot for the only piece of its tile.
+// spread: the tile's first kSpread columns only, by all four wavefronts, each with a quarter of the
+// rows: the sinks, which every later row sees.
 struct KeyPiece {
     uint32_t key0, nkey, row0, nrow;
     int32_t pos0, col0;
-    uint32_t slot, pad;
+    uint32_t step0, nsteps, slot, spread, pad[2];
 };
+constexpr uint32_t kRowStep = 64, kSpread = 32;
 
-// A tile of columns in several pieces: partial sums first .. first + count.
+// A tile of columns in several pieces: partial sums first .. first + count, then `spread` ones of
+// its first columns.
 struct KeySplit {
-    uint32_t key0, nkey, first, count;
+    uint32_t key0, nkey, first, count, spread, pad[3];
 };
 
 struct BandArgs {

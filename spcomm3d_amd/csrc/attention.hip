@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
 
     const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
     const RowTile t = a.tiles[w.tile];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
     const int dim = (int)a.dim, ncols = (int)t.ncols;
     const uint32_t kvh = w.head / (a.heads / a.kv_heads);
     const T *const qp = (const T *)a.q.p + t.row0 * a.q.stride + w.head * dim;
@@ -80,11 +80,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
     const T *const vp = (const T *)a.v.p + t.key0 * a.v.stride + kvh * dim;
 
     Frag<T> qf[NQ][NS];
-    int pos[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int r = (wave * NQ + n) * 16 + l;
-        pos[n] = t.pos0 + r;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int d = 32 * s + 8 * g;
@@ -123,7 +121,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
         for (int k = 0; k < st.count; ++k) {
             const int c0 = st.at(k) * (int)kKeyStep;
             char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
-            const int lane = fresh(tid & 63);
+            const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
             loads_done();
             __syncthreads();
             if (k + 1 < st.count)
@@ -154,7 +152,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
                     for (int n = 0; n < NQ; ++n)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (!sees(pos[n], c0 + 16 * i + 4 * g + j, a.window, a.sinks))
+                            if (!sees(wa + 16 * n + l, c0 + 16 * i + 4 * g + j, a.window, a.sinks))
                                 sv[i][n][j] = kNegInf;
             }
             float top[NQ];
@@ -230,7 +228,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
                             if (!is_finite(x)) {
 #pragma unroll
                                 for (int n = 0; n < NQ; ++n)
-                                    if (sees(pos[n], c0 + c, a.window, a.sinks))
+                                    if (sees(wa + 16 * n + l, c0 + c, a.window, a.sinks))
                                         acc[d][n][j] += (float)x;
                             }
                         }
@@ -284,7 +282,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
 
     const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
     const RowTile t = a.tiles[w.tile];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
     const int dim = (int)a.dim, ncols = (int)t.ncols;
     const uint32_t kvh = w.head / (a.heads / a.kv_heads);
     const T *const qp = (const T *)a.q.p + t.row0 * a.q.stride + w.head * dim;
@@ -294,13 +292,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
     const T *const vp = (const T *)a.v.p + t.key0 * a.v.stride + kvh * dim;
 
     Frag<T> qf[NQ][NS], gf[NQ][NS];
-    int pos[NQ];
     float lse[NQ], delta[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int r = (wave * NQ + n) * 16 + l;
         const bool mine = r < (int)t.nrow;
-        pos[n] = t.pos0 + r;
         float dot = 0.0f;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -350,7 +346,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
         for (int k = 0; k < st.count; ++k) {
             const int c0 = st.at(k) * (int)kKeyStep;
             char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
-            const int lane = fresh(tid & 63);
+            const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
             loads_done();
             __syncthreads();
             if (k + 1 < st.count)
@@ -383,7 +379,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
                         for (int n = 0; n < NQ; ++n)
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                if (!sees(pos[n], c0 + 32 * u + 16 * i + 4 * g + j, a.window, a.sinks)) {
+                                if (!sees(wa + 16 * n + l, c0 + 32 * u + 16 * i + 4 * g + j, a.window, a.sinks)) {
                                     sv[n][j] = kNegInf;
                                     dp[n][j] = 0.0f;
                                 }
@@ -451,7 +447,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_kernel(BandArgs a)
 {
     typedef Tile<T, DP> L;
-    constexpr int NS = DP / 32, ND = DP / 16, NK = 2, ROWS = 64;
+    constexpr int NS = DP / 32, ND = DP / 16, NK = 2, ROWS = kRowStep;
     constexpr float kUp = sizeof(T) == 2 && WeightShift<T>::value != 0 ? 32768.0f : 1.0f; // weights are at most 1 here
     constexpr int kBytes = ROWS * L::kRowBytes;
     __shared__ __align__(16) char tiles[2][2][kBytes]; // Q and dO of this step and the next
@@ -460,18 +456,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
     const uint32_t group = a.heads / a.kv_heads;
     const Work w = work_of(blockIdx.x, a.npieces, a.kv_heads, a.kv_heads);
     const KeyPiece t = a.pieces[w.tile];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
     const int dim = (int)a.dim, nrow = (int)t.nrow;
     const T *const kp = (const T *)a.k.p + t.key0 * a.k.stride + w.head * dim;
     const T *const vp = (const T *)a.v.p + t.key0 * a.v.stride + w.head * dim;
 
     Frag<T> kf[NK][NS], vf[NK][NS];
     f32x4 dk[NK][ND], dv[NK][ND];
-    int col[NK];
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
-        const int r = (wave * NK + n) * 16 + l;
-        col[n] = t.col0 + r;
+        const int r = ((t.spread ? 0 : wave * NK) + n) * 16 + l;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int d = 32 * s + 8 * g;
@@ -483,10 +477,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
         for (int d = 0; d < ND; ++d)
             dk[n][d] = dv[n][d] = f32x4{0, 0, 0, 0};
     }
-    const int wave_first = __builtin_amdgcn_readfirstlane(wave * NK * 16);
+    const int wave_first = t.spread ? 0 : wave * NK * 16; // its first column
     const int ca = t.col0 + wave_first, cb = ca + NK * 16 - 1;
     const float sc = a.scale * kLog2e;
-    const int per = (nrow + ROWS - 1) / ROWS, count = per * (int)group;
+    const int per = (nrow + ROWS - 1) / ROWS, first = (int)t.step0, end = first + (int)t.nsteps;
 
     if (dim < DP)
         clear_tile<4 * kBytes, kThreads>(tiles[0][0], tid);
@@ -509,15 +503,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
         }
     };
     __syncthreads();
-    if (count > 0)
-        fetch(0);
-    for (int k = 0; k < count; ++k) {
+    if (first < end)
+        fetch(first);
+    for (int k = first; k < end; ++k) {
         char *const qt = tiles[k & 1][0], *const gt = tiles[k & 1][1];
         const float *const stat = stats[k & 1];
-        const int lane = fresh(tid & 63);
+        const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
         loads_done();
         __syncthreads();
-        if (k + 1 < count)
+        if (k + 1 < end)
             fetch(k + 1);
         const int pa = t.pos0 + (k % per) * ROWS, pb = pa + ROWS - 1;
         if (pb < ca || (pa - cb >= a.window && ca >= a.sinks))
@@ -526,6 +520,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
 
 #pragma unroll
         for (int u = 0; u < ROWS / 32; ++u) {
+            if (t.spread && ((2 * k + u) & 3) != wave)
+                continue;
             HalfFrag<T> ps[2][NK], ds[2][NK];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -550,7 +546,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
                     for (int n = 0; n < NK; ++n)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (!sees(pa + 32 * u + 16 * i + 4 * g + j, col[n], a.window, a.sinks)) {
+                            if (!sees(pa + 32 * u + 16 * i + 4 * g + j, ca + 16 * n + l, a.window, a.sinks)) {
                                 sv[n][j] = kNegInf;
                                 dp[n][j] = 0.0f;
                             }
@@ -596,8 +592,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int c = (wave * NK + n) * 16 + 4 * g + j;
-            if (c >= (int)t.nkey)
-                continue;
+            if (!t.spread && c >= (int)t.nkey)
+                continue; // (spread: places of the slot, whose columns past nkey nobody reads)
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const int e = 16 * d + l;
@@ -628,6 +624,12 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_dkv_kerne
             x += part[s * step + i];
             y += part[s * step + kKeyTile * dim + i];
         }
+        if (c < kSpread)
+            for (uint32_t s = t.count; s < t.count + t.spread; ++s)
+                for (uint32_t w = 0; w < kKeyTile; w += kSpread) { // one part of each wavefront
+                    x += part[s * step + w * dim + i];
+                    y += part[s * step + (kKeyTile + w) * dim + i];
+                }
         ((T *)a.dk.p)[(t.key0 + c) * a.dk.stride + h * dim + e] = (T)(x * a.scale);
         ((T *)a.dv.p)[(t.key0 + c) * a.dv.stride + h * dim + e] = (T)y;
     }
