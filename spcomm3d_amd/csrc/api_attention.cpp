@@ -11,9 +11,9 @@
 
 namespace {
 
-// The pieces that spc3d_attend_grad's column kernel works on, for one number of heads.
+// The pieces that spc3d_attend_grad's column kernel works on, for one number and kind of heads.
 struct KeySchedule {
-    uint32_t kv_heads = 0, group = 0, npieces = 0, nsplits = 0, nslots = 0;
+    uint32_t kv_heads = 0, group = 0, row_step = 0, npieces = 0, nsplits = 0, nslots = 0;
     KeyPiece *pieces = nullptr;
     KeySplit *splits = nullptr;
 };
@@ -127,11 +127,11 @@ uint64_t makespan(const std::vector<uint64_t> &costs, size_t slots)
 
 // Tiles of kKeyTile columns, each with the rows that see one of them, cut into pieces of steps
 // where that ends sooner.  Rows that see a tile for its sinks alone are pieces of their own.
-// The choice goes by what the parts of a call cost on an MI355X, in steps of kRowStep rows (7 us with
+// The choice goes by what the parts of a call cost on an MI355X, in steps (64 rows, 7 us with
 // two workgroups on a CU, heads of 128 in 16 bits): half a step to begin and end a piece, two more
 // to write its partial sums, half a step of the whole GPU for the launch that joins them and 1/512
 // for each piece in it.
-void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, std::vector<KeyPiece> &pieces,
+void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, uint32_t row_step, std::vector<KeyPiece> &pieces,
                 std::vector<KeySplit> &splits, uint32_t *nslots)
 {
     std::vector<KeyPiece> tiles;
@@ -141,7 +141,7 @@ void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, std::vec
         t.row0 = row0 + (uint32_t)lo;
         t.nrow = (uint32_t)std::max<int64_t>(0, hi - lo);
         t.pos0 = (int32_t)(lo + off);
-        t.nsteps = (t.nrow + kRowStep - 1) / kRowStep * group;
+        t.nsteps = (t.nrow + row_step - 1) / row_step * group;
         t.slot = kNoSlot;
         longest = std::max<uint64_t>(longest, t.nsteps);
         tiles.push_back(t);
@@ -168,7 +168,7 @@ void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, std::vec
     // the longest piece allowed, by trial
     const size_t slots = std::max<size_t>(1, 2 * (size_t)b->ctx->cu_count / kv_heads);
     auto count_of = [&](const KeyPiece &t, uint64_t most) {
-        const uint64_t all = t.spread ? (t.nsteps + 1) / 2 : t.nsteps; // a spread step costs half of one
+        const uint64_t all = t.spread ? (t.nsteps * 5ull + 7) / 8 : t.nsteps; // a step of the sinks costs five eighths
         return (uint32_t)std::max<uint64_t>(1, (all + most - 1) / most);
     };
     uint64_t best = longest, best_cost = UINT64_MAX;
@@ -183,7 +183,7 @@ void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, std::vec
             const KeyPiece &t = tiles[i];
             const uint32_t count = count_of(t, most);
             const bool split = count > 1 || t.spread || (i + 1 < tiles.size() && tiles[i + 1].spread);
-            const uint64_t each = 512ull * t.nsteps / count / (t.spread ? 2 : 1);
+            const uint64_t each = 512ull * t.nsteps * row_step / 64 * (t.spread ? 5 : 8) / 8 / count;
             for (uint32_t k = 0; k < count; ++k)
                 costs.push_back(each + 256 + (split ? 1024 : 0));
             joined += split ? count : 0;
@@ -213,7 +213,7 @@ void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, std::vec
             p.nsteps = (uint32_t)((uint64_t)t.nsteps * (k + 1) / count) - p.step0;
             if (!lone)
                 p.slot = next++;
-            all.push_back({t.spread ? p.nsteps / 2 : p.nsteps, p});
+            all.push_back({t.spread ? p.nsteps * 5ull / 8 : p.nsteps, p});
         }
     }
     std::stable_sort(all.begin(), all.end(), [](const auto &x, const auto &y) { return x.first > y.first; });
@@ -222,10 +222,10 @@ void key_pieces(const spc3d_band *b, uint32_t kv_heads, uint32_t group, std::vec
     *nslots = next;
 }
 
-int schedule_of(spc3d_band *b, uint32_t kv_heads, uint32_t group, KeySchedule **out)
+int schedule_of(spc3d_band *b, uint32_t kv_heads, uint32_t group, uint32_t row_step, KeySchedule **out)
 {
     for (KeySchedule &s : b->schedules)
-        if (s.kv_heads == kv_heads && s.group == group) {
+        if (s.kv_heads == kv_heads && s.group == group && s.row_step == row_step) {
             *out = &s;
             return SPC3D_OK;
         }
@@ -234,10 +234,11 @@ int schedule_of(spc3d_band *b, uint32_t kv_heads, uint32_t group, KeySchedule **
     KeySchedule s;
     s.kv_heads = kv_heads;
     s.group = group;
+    s.row_step = row_step;
     std::vector<KeyPiece> pieces;
     std::vector<KeySplit> splits;
     try {
-        key_pieces(b, kv_heads, group, pieces, splits, &s.nslots);
+        key_pieces(b, kv_heads, group, row_step, pieces, splits, &s.nslots);
         b->schedules.reserve(b->schedules.size() + 1);
     } catch (const std::bad_alloc &) {
         return fail(SPC3D_ERR_ALLOC, "host allocation failed");
@@ -513,7 +514,8 @@ int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q, co
     if (rc)
         return rc;
     KeySchedule *s = nullptr;
-    rc = schedule_of(band, k->heads, q->heads / k->heads, &s);
+    rc = schedule_of(band, k->heads, q->heads / k->heads,
+                     dkv_row_step((uint32_t)elem_size(dt), padded_dim((uint32_t)elem_size(dt), q->dim)), &s);
     if (rc)
         return rc;
     if ((uint64_t)s->npieces * k->heads > INT_MAX || s->nsplits > INT_MAX || k->heads > 65535)

@@ -27,17 +27,23 @@ struct RowTile {
 
 // A piece of a tile of columns: columns col0 .. col0 + nkey of their sequence, rows key0 .. of the
 // packed keys.  The rows row0 .. row0 + nrow (from position pos0 on) of every head that shares the
-// columns see some of them; in steps of kRowStep rows, head after head, this piece takes the steps
+// columns see some of them; in steps of dkv_row_step rows, head after head, this piece takes the steps
 // step0 .. step0 + nsteps.
 // slot: where its partial sums go, or kNoSlot for the only piece of its tile.
-// spread: the tile's first kSpread columns only, by all four wavefronts, each with a quarter of the
-// rows: the sinks, which every later row sees.
+// spread: the tile's first kSpread columns only, by all four wavefronts, each with a quarter of a
+// head's elements: the sinks, which every later row sees.
 struct KeyPiece {
     uint32_t key0, nkey, row0, nrow;
     int32_t pos0, col0;
     uint32_t step0, nsteps, slot, spread, pad[2];
 };
-constexpr uint32_t kRowStep = 64, kSpread = 32;
+constexpr uint32_t kSpread = 16;
+// Whether a wavefront of the column kernel has registers for its values, and the rows of a step,
+// for elements of `size` bytes and heads computed as `width` of them.
+constexpr bool dkv_keeps_v(uint32_t size, uint32_t width) { return size == 4 || width < 128; }
+constexpr uint32_t dkv_row_step(uint32_t size, uint32_t width) { return dkv_keeps_v(size, width) ? 64 : 32; }
+// Elements that heads of `dim` are computed as, zeros behind their own.
+constexpr uint32_t padded_dim(uint32_t size, uint32_t dim) { return dim <= 64 ? 64 : (dim <= 96 && size == 2 ? 96 : 128); }
 
 // A tile of columns in several pieces: partial sums first .. first + count, then `spread` ones of
 // its first columns.

@@ -15,6 +15,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kFewSteps = 2;
 
+// In a block that few steps enter: as selects instead of a branch, masks would cost every step as much
+// as its exponentials.
+#define KEEP_BRANCH() asm volatile("")
+
 struct Work {
     uint32_t tile, head;
 };
@@ -68,7 +72,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
     typedef Tile<T, DP> L;
     constexpr int NS = DP / 32, ND = DP / 16, NT = kKeyStep / 16;
     constexpr int kBytes = kKeyStep * L::kRowBytes;
-    __shared__ __align__(16) char tiles[2][2][kBytes]; // keys and values of this step and the next
+    // Keys, then values, of this step and of the next.  Two arrays and every other step its own
+    // code: the compiler then knows that the reads of one do not wait for the loads of the other.
+    __shared__ __align__(16) char even[2 * kBytes], odd[2 * kBytes];
 
     const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
     const RowTile t = a.tiles[w.tile];
@@ -92,11 +98,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
     const Steps st = steps_of(t.pos0, t.pos0 + (int)t.nrow - 1, ncols, a.window, a.sinks);
     const int wa = t.pos0 + wave * NQ * 16, wb = min(wa + NQ * 16, t.pos0 + (int)t.nrow) - 1;
     const float sc = a.scale * kLog2e;
-    if (dim < DP)
-        clear_tile<4 * kBytes, kThreads>(tiles[0][0], tid);
-    auto fetch = [&](int k) {
+    if (dim < DP) {
+        clear_tile<2 * kBytes, kThreads>(even, tid);
+        clear_tile<2 * kBytes, kThreads>(odd, tid);
+    }
+    auto fetch = [&](int k, char *kt) {
         const int c0 = st.at(k) * (int)kKeyStep;
-        char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+        char *const vt = kt + kBytes;
         const int id = fresh(tid);
         load_tile<T, DP, kKeyStep, kThreads>(kt, kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, id);
         load_tile<T, DP, kKeyStep, kThreads>(vt, vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, id);
@@ -106,7 +114,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
     float m[NQ], sum[NQ];
     // The second pass, if any, is for values that are not finite: 0 x inf would reach rows that do
     // not see them, so steps with hidden pairs take those values one by one.
-    auto pass = [&](auto careful) {
+    auto pass = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             m[n] = kNegInf;
@@ -117,18 +125,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
         }
         __syncthreads(); // the tiles are cleared, or read for the last time
         if (st.count > 0)
-            fetch(0);
-        for (int k = 0; k < st.count; ++k) {
+            fetch(0, even);
+        auto step = [&](int k, char *kt, char *next) __attribute__((always_inline)) {
             const int c0 = st.at(k) * (int)kKeyStep;
-            char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+            char *const vt = kt + kBytes;
             const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
             loads_done();
             __syncthreads();
             if (k + 1 < st.count)
-                fetch(k + 1);
+                fetch(k + 1, next);
             const int c9 = c0 + (int)kKeyStep - 1;
             if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
-                continue; // nothing here is seen by this wavefront's rows
+                return; // nothing here is seen by this wavefront's rows
             const bool whole = c9 <= wa && (wb - c0 < a.window || c9 < a.sinks);
 
             f32x4 sv[NT][NQ];
@@ -146,6 +154,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
                 }
             }
             if (!whole) {
+                KEEP_BRANCH();
 #pragma unroll
                 for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -233,6 +242,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
                             }
                         }
             }
+        };
+        for (int k = 0; k < st.count; k += 2) {
+            step(k, even, odd);
+            if (k + 1 < st.count)
+                step(k + 1, odd, even);
         }
         int bad = 0;
 #pragma unroll
@@ -278,7 +292,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
     typedef Tile<T, DP> L;
     constexpr int NS = DP / 32, ND = DP / 16, NT = kKeyStep / 16;
     constexpr int kBytes = kKeyStep * L::kRowBytes;
-    __shared__ __align__(16) char tiles[2][2][kBytes]; // keys and values of this step and the next
+    // Keys, then values, of this step and of the next.  Two arrays and every other step its own
+    // code: the compiler then knows that the reads of one do not wait for the loads of the other.
+    __shared__ __align__(16) char even[2 * kBytes], odd[2 * kBytes];
 
     const Work w = work_of(blockIdx.x, a.ntiles, a.heads, a.kv_heads);
     const RowTile t = a.tiles[w.tile];
@@ -317,11 +333,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
     const Steps st = steps_of(t.pos0, t.pos0 + (int)t.nrow - 1, ncols, a.window, a.sinks);
     const int wa = t.pos0 + wave * NQ * 16, wb = min(wa + NQ * 16, t.pos0 + (int)t.nrow) - 1;
     const float sc = a.scale * kLog2e;
-    if (dim < DP)
-        clear_tile<4 * kBytes, kThreads>(tiles[0][0], tid);
-    auto fetch = [&](int k) {
+    if (dim < DP) {
+        clear_tile<2 * kBytes, kThreads>(even, tid);
+        clear_tile<2 * kBytes, kThreads>(odd, tid);
+    }
+    auto fetch = [&](int k, char *kt) {
         const int c0 = st.at(k) * (int)kKeyStep;
-        char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+        char *const vt = kt + kBytes;
         const int id = fresh(tid);
         load_tile<T, DP, kKeyStep, kThreads>(kt, kp + c0 * a.k.stride, a.k.stride, ncols - c0, dim, id);
         load_tile<T, DP, kKeyStep, kThreads>(vt, vp + c0 * a.v.stride, a.v.stride, ncols - c0, dim, id);
@@ -332,7 +350,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
     // Rows that see few columns take it before they use it: their dS is a small difference, and
     // the rounding of o in <dO, o> would show (dQ of 300 rows in bfloat16: 1.72 times the error of
     // one rounding, 1.47 so; further down the sequence it is lost among the columns).
-    auto pass = [&](auto last) {
+    auto pass = [&](auto last) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             weighed[n] = 0.0f;
@@ -342,18 +360,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
         }
         __syncthreads(); // the tiles are cleared, or read for the last time
         if (st.count > 0)
-            fetch(0);
-        for (int k = 0; k < st.count; ++k) {
+            fetch(0, even);
+        auto step = [&](int k, char *kt, char *next) __attribute__((always_inline)) {
             const int c0 = st.at(k) * (int)kKeyStep;
-            char *const kt = tiles[k & 1][0], *const vt = tiles[k & 1][1];
+            char *const vt = kt + kBytes;
             const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
             loads_done();
             __syncthreads();
             if (k + 1 < st.count)
-                fetch(k + 1);
+                fetch(k + 1, next);
             const int c9 = c0 + (int)kKeyStep - 1;
             if (wb < c0 || (wa - c9 >= a.window && c0 >= a.sinks))
-                continue;
+                return;
             const bool whole = c9 <= wa && (wb - c0 < a.window || c9 < a.sinks);
 #pragma unroll
             for (int u = 0; u < NT / 2; ++u) {
@@ -375,6 +393,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
                         }
                     }
                     if (!whole) {
+                KEEP_BRANCH();
 #pragma unroll
                         for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -409,6 +428,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
                     }
                 }
             }
+        };
+        for (int k = 0; k < st.count; k += 2) {
+            step(k, even, odd);
+            if (k + 1 < st.count)
+                step(k + 1, odd, even);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -439,19 +463,24 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_ke
     }
 }
 
-// Each wavefront owns 32 columns of the tile's 128, whose keys and values stay in its registers;
-// rows (of every head that shares them) come through LDS 64 at a time.  S = Q K^T leaves a lane
+// Each wavefront owns 32 columns of the tile's 128, whose keys and values stay in its registers
+// (values of the largest heads in LDS: two wavefronts to a SIMD have room for the sums, the keys and
+// some fragments ahead, and no more);
+// rows (of every head that shares them) come through LDS 64 (32) at a time.  S = Q K^T leaves a lane
 // with one column and the rows 4 g + i, 16 + 4 g + i, which is the left operand of dV += P^T dO and
 // dK += dS^T Q as it lies.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_kernel(BandArgs a)
 {
     typedef Tile<T, DP> L;
-    constexpr int NS = DP / 32, ND = DP / 16, NK = 2, ROWS = kRowStep;
+    constexpr int NS = DP / 32, ND = DP / 16, NK = 2;
+    constexpr bool kKeepV = dkv_keeps_v(sizeof(T), DP);
+    constexpr int ROWS = dkv_row_step(sizeof(T), DP);
     constexpr float kUp = sizeof(T) == 2 && WeightShift<T>::value != 0 ? 32768.0f : 1.0f; // weights are at most 1 here
     constexpr int kBytes = ROWS * L::kRowBytes;
-    __shared__ __align__(16) char tiles[2][2][kBytes]; // Q and dO of this step and the next
-    __shared__ __align__(16) float stats[2][2 * ROWS]; // lse and <dO, o> of their rows
+    // Q, then dO, then lse and <dO, o> of the rows
+    __shared__ __align__(16) char even[2 * kBytes + 8 * ROWS], odd[2 * kBytes + 8 * ROWS];
+    __shared__ __align__(16) char values[kKeepV ? 16 : kKeyTile * L::kRowBytes];
 
     const uint32_t group = a.heads / a.kv_heads;
     const Work w = work_of(blockIdx.x, a.npieces, a.kv_heads, a.kv_heads);
@@ -461,7 +490,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
     const T *const kp = (const T *)a.k.p + t.key0 * a.k.stride + w.head * dim;
     const T *const vp = (const T *)a.v.p + t.key0 * a.v.stride + w.head * dim;
 
-    Frag<T> kf[NK][NS], vf[NK][NS];
+    Frag<T> kf[NK][NS], vf[NK][kKeepV ? NS : 1];
     f32x4 dk[NK][ND], dv[NK][ND];
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
@@ -471,21 +500,31 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
             const int d = 32 * s + 8 * g;
             const bool in = r < (int)t.nkey && d < dim;
             kf[n][s] = in ? load_frag(kp + r * a.k.stride + d) : zero_frag<T>();
-            vf[n][s] = in ? load_frag(vp + r * a.v.stride + d) : zero_frag<T>();
+            if constexpr (kKeepV)
+                vf[n][s] = in ? load_frag(vp + r * a.v.stride + d) : zero_frag<T>();
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d)
             dk[n][d] = dv[n][d] = f32x4{0, 0, 0, 0};
     }
     const int wave_first = t.spread ? 0 : wave * NK * 16; // its first column
-    const int ca = t.col0 + wave_first, cb = ca + NK * 16 - 1;
+    const int ca = t.col0 + wave_first, cb = ca + (t.spread ? (int)kSpread : NK * 16) - 1;
     const float sc = a.scale * kLog2e;
     const int per = (nrow + ROWS - 1) / ROWS, first = (int)t.step0, end = first + (int)t.nsteps;
 
-    if (dim < DP)
-        clear_tile<4 * kBytes, kThreads>(tiles[0][0], tid);
-    auto fetch = [&](int k) {
-        char *const qt = tiles[k & 1][0], *const gt = tiles[k & 1][1];
+    if (dim < DP) {
+        clear_tile<2 * kBytes, kThreads>(even, tid);
+        clear_tile<2 * kBytes, kThreads>(odd, tid);
+        if constexpr (!kKeepV) {
+            clear_tile<kKeyTile * L::kRowBytes, kThreads>(values, tid);
+            __syncthreads();
+        }
+    }
+    if constexpr (!kKeepV)
+        if (first < end) // no load may outlive its workgroup
+            load_tile<T, DP, kKeyTile, kThreads>(values, vp, a.v.stride, (int)t.nkey, dim, tid);
+    auto fetch = [&](int k, char *qt) {
+        char *const gt = qt + kBytes;
         const uint32_t head = w.head * group + k / per;
         const int r0 = (k % per) * ROWS;
         const uint64_t row = t.row0 + r0;
@@ -494,34 +533,36 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
                                          dim, id);
         load_tile<T, DP, ROWS, kThreads>(gt, (const T *)a.d_o.p + row * a.d_o.stride + head * dim, a.d_o.stride,
                                          nrow - r0, dim, id);
-        const int which = __builtin_amdgcn_readfirstlane(id >> 6);
-        if (which < 2) { // rows past the end weigh nothing
-            const int r = id & 63;
+        const int part = __builtin_amdgcn_readfirstlane(id >> 6);
+        if (part * 64 < 2 * ROWS) { // rows past the end weigh nothing
+            const int r = id % ROWS;
             const uint64_t at = r0 + r < nrow ? (row + r) * a.heads + head : a.nstats - 1;
-            __builtin_amdgcn_global_load_lds((global_void *)(a.stats + which * a.nstats + at),
-                                             (lds_void *)(stats[k & 1] + which * ROWS), 4, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_void *)(a.stats + id / ROWS * a.nstats + at),
+                                             (lds_void *)(gt + kBytes + part * 256), 4, 0, 0);
         }
     };
     __syncthreads();
     if (first < end)
-        fetch(first);
-    for (int k = first; k < end; ++k) {
-        char *const qt = tiles[k & 1][0], *const gt = tiles[k & 1][1];
-        const float *const stat = stats[k & 1];
+        fetch(first, even);
+    // A piece of the sinks: every wavefront has the same 16 columns (n = 0) and sums its own
+    // quarter of the elements, dk[0][d] then being element 16 (wave kQuarter + d) + l.
+    constexpr int kQuarter = (ND + 3) / 4;
+    auto step = [&](auto spread, int k, char *qt, char *next) __attribute__((always_inline)) {
+        constexpr int NK = spread.value ? 1 : 2;
+        char *const gt = qt + kBytes;
+        const float *const stat = (const float *)(gt + kBytes);
         const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
         loads_done();
         __syncthreads();
         if (k + 1 < end)
-            fetch(k + 1);
+            fetch(k + 1, next);
         const int pa = t.pos0 + (k % per) * ROWS, pb = pa + ROWS - 1;
         if (pb < ca || (pa - cb >= a.window && ca >= a.sinks))
-            continue;
+            return;
         const bool whole = pa >= cb && (pb - ca < a.window || cb < a.sinks);
 
 #pragma unroll
         for (int u = 0; u < ROWS / 32; ++u) {
-            if (t.spread && ((2 * k + u) & 3) != wave)
-                continue;
             HalfFrag<T> ps[2][NK], ds[2][NK];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -536,12 +577,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
 #pragma unroll
                     for (int n = 0; n < NK; ++n) {
                         sv[n] = mma(f, kf[n][s], sv[n]);
-                        dp[n] = mma(h, vf[n][s], dp[n]);
+                        dp[n] = mma(h, kKeepV ? vf[n][kKeepV ? s : 0] : L::rows(values, wave_first + 16 * n, s, lane),
+                                    dp[n]);
                     }
                 }
                 const f32x4 lse = *reinterpret_cast<const f32x4 *>(stat + 32 * u + 16 * i + 4 * g);
                 const f32x4 delta = *reinterpret_cast<const f32x4 *>(stat + ROWS + 32 * u + 16 * i + 4 * g);
                 if (!whole) {
+                KEEP_BRANCH();
 #pragma unroll
                     for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -570,9 +613,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
                 df[n] = join<T>(ds[0][n], ds[1][n]);
             }
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const Frag<T> f = L::columns(gt, 32 * u, d, lane);
-                const Frag<T> h = L::columns(qt, 32 * u, d, lane);
+            for (int d = 0; d < (spread.value ? kQuarter : ND); ++d) {
+                const int dd = spread.value ? wave * kQuarter + d : d;
+                // (a quarter past the last element takes that one again: nobody reads its sums)
+                const Frag<T> f = L::columns(gt, 32 * u, spread.value ? min(dd, ND - 1) : dd, lane);
+                const Frag<T> h = L::columns(qt, 32 * u, spread.value ? min(dd, ND - 1) : dd, lane);
 #pragma unroll
                 for (int n = 0; n < NK; ++n) {
                     dv[n][d] = mma(pf[n], f, dv[n][d]);
@@ -580,20 +625,44 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
                 }
             }
         }
-    }
+    };
+    auto walk = [&](auto spread) __attribute__((always_inline)) {
+        for (int k = first; k < end; k += 2) {
+            step(spread, k, even, odd);
+            if (k + 1 < end)
+                step(spread, k + 1, odd, even);
+        }
+    };
+    if (t.spread)
+        walk(std::true_type());
+    else
+        walk(std::false_type());
     // lane l holds element 16 d + l of the columns 4 g + j
     T *const dkp = (T *)a.dk.p + t.key0 * a.dk.stride + w.head * dim;
     T *const dvp = (T *)a.dv.p + t.key0 * a.dv.stride + w.head * dim;
     float *const part = t.slot == kNoSlot
                             ? nullptr
                             : a.partial + ((uint64_t)t.slot * a.kv_heads + w.head) * 2 * kKeyTile * dim;
+    if (t.spread) {
+#pragma unroll
+        for (int d = 0; d < kQuarter; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = 4 * g + j, e = 16 * (wave * kQuarter + d) + l;
+                if (c < (int)t.nkey && e < dim) {
+                    part[c * dim + e] = dk[0][d][j];
+                    part[(kKeyTile + c) * dim + e] = dv[0][d][j] * (1.0f / kUp);
+                }
+            }
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int c = (wave * NK + n) * 16 + 4 * g + j;
-            if (!t.spread && c >= (int)t.nkey)
-                continue; // (spread: places of the slot, whose columns past nkey nobody reads)
+            if (c >= (int)t.nkey)
+                continue;
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const int e = 16 * d + l;
@@ -620,16 +689,10 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_dkv_kerne
     for (uint32_t i = blockIdx.z * kThreads + threadIdx.x; i < t.nkey * dim; i += gridDim.z * kThreads) {
         const uint32_t c = i / dim, e = i % dim;
         float x = 0.0f, y = 0.0f;
-        for (uint32_t s = 0; s < t.count; ++s) {
+        for (uint32_t s = 0; s < t.count + (c < kSpread ? t.spread : 0); ++s) {
             x += part[s * step + i];
             y += part[s * step + kKeyTile * dim + i];
         }
-        if (c < kSpread)
-            for (uint32_t s = t.count; s < t.count + t.spread; ++s)
-                for (uint32_t w = 0; w < kKeyTile; w += kSpread) { // one part of each wavefront
-                    x += part[s * step + w * dim + i];
-                    y += part[s * step + (kKeyTile + w) * dim + i];
-                }
         ((T *)a.dk.p)[(t.key0 + c) * a.dk.stride + h * dim + e] = (T)(x * a.scale);
         ((T *)a.dv.p)[(t.key0 + c) * a.dv.stride + h * dim + e] = (T)y;
     }
@@ -664,10 +727,9 @@ template <typename T, int DP> void launch_one(const BandArgs &a, Op op, uint32_t
         hipLaunchKernelGGL((attend_kernel<T, DP, 1>), rows, block, 0, s, a);
 }
 
-// Heads are computed as if they had 64, 96 or 128 elements (32 bits: 64 or 128), zeros behind their own.
 hipError_t launch(const BandArgs &a, Op op, uint32_t tile_rows, hipStream_t s)
 {
-    const int dp = a.dim <= 64 ? 64 : (a.dim <= 96 && a.dtype != 0 ? 96 : 128);
+    const int dp = (int)padded_dim(a.dtype == 0 ? 4 : 2, a.dim);
     switch (a.dtype * 1000 + dp) {
     case 64: launch_one<float, 64>(a, op, tile_rows, s); break;
     case 128: launch_one<float, 128>(a, op, tile_rows, s); break;
