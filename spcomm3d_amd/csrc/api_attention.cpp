@@ -800,16 +800,16 @@ int spc3d_cache_attend(spc3d_ctx *ctx, spc3d_cache *cache, const spc3d_cache_seq
     const uint32_t group = q->heads / a.c.heads, cols = read_columns(a.s.max_rows, group);
     const uint64_t tiles = ((uint64_t)a.s.max_rows * group + cols - 1) / cols;
     const uint64_t groups = (uint64_t)seqs->nseq * tiles * a.c.heads;
-    // Workgroups for two on each CU, as far as each gets two steps of 64 tokens for every one of
-    // its four wavefronts.
-    uint64_t steps = ((uint64_t)seqs->max_len + kKeyStep - 1) / kKeyStep;
+    // Shares of a sequence's steps: such that the longest sequences would make eight workgroups for each
+    // CU (of sequences of several lengths most are shorter, and a share that has no tokens ends at
+    // once), but at least a step for each of a workgroup's four wavefronts.
+    const uint64_t step = read_step(a.c.dtype);
+    uint64_t steps = ((uint64_t)seqs->max_len + step - 1) / step;
     if (a.window != INT_MAX)
-        steps = std::min(steps, ((uint64_t)window + a.s.max_rows + kKeyStep - 1) / kKeyStep + 1 +
-                                    ((uint64_t)a.sinks + kKeyStep - 1) / kKeyStep);
-    const uint64_t want = 2ull * ctx->cu_count;
-    a.splits = 1;
-    if (groups && groups < want)
-        a.splits = (uint32_t)std::max<uint64_t>(1, std::min((want + groups - 1) / groups, steps / 8));
+        steps = std::min(steps, ((uint64_t)window + a.s.max_rows + step - 1) / step + 1 + ((uint64_t)a.sinks + step - 1) / step);
+    const uint64_t share = groups * steps / (8ull * ctx->cu_count);
+    a.share = (uint32_t)std::max<uint64_t>(4, (share + 3) / 4 * 4);
+    a.splits = (uint32_t)std::max<uint64_t>(1, (steps + a.share - 1) / a.share);
     a.col_tiles = (uint32_t)tiles;
     if (groups * a.splits > INT_MAX || (uint64_t)seqs->rows * q->heads / 8 > INT_MAX)
         return fail(SPC3D_ERR_TOO_LARGE, "more rows and heads than a grid holds");

@@ -42,12 +42,14 @@ struct ReadArgs {
     int dtype;
     uint32_t col_tiles;  // tiles of 16 * columns_per_wave (row, head) pairs of a kv head
     uint32_t splits;     // workgroups that share the tokens of a sequence
+    uint32_t share;      // steps of read_step() tokens that each of them has at most
     float *partial;      // [row][head][split][dim + 2], with more than one
 };
 
 hipError_t launch_cache_append(const AppendArgs &a, hipStream_t stream);
 // (row, head) pairs that a workgroup takes: 16 or 32.
 uint32_t read_columns(uint32_t max_rows, uint32_t group);
+uint32_t read_step(int cache_dtype);
 hipError_t launch_cache_read(const ReadArgs &a, hipStream_t stream);
 
 } // namespace spc3d

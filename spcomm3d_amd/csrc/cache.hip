@@ -3,6 +3,8 @@
 #include "cache.h"
 #include "attention_frag.h"
 
+#include <type_traits>
+
 namespace spc3d {
 namespace {
 
@@ -250,18 +252,14 @@ template <typename T, typename C> __global__ __launch_bounds__(kThreads) void ap
 
 // ---- read -------------------------------------------------------------------------------------
 // Columns are the (row, head) pairs that share a kv head, 16 NC of them a workgroup; its four
-// wavefronts take 64 tokens at a time, in turn, each with its own running maximum and sum, joined
+// wavefronts take the steps of its share of the tokens in turn, each with its own running maximum and sum, joined
 // at the end.  Nothing goes through LDS on the way: S^T = K Q^T wants a token's elements, O^T =
-// V^T P^T an element's tokens, and that is how the cache holds them.  Which token stands in which
-// row of S^T is free; they are dealt so that a lane's probabilities are the tokens 16 g .. 16 g + 15
+// V^T P^T an element's tokens, and that is how the cache holds them.  A lane loads 16 bytes, so a
+// step has 4 kTok tokens, kTok of them (16 in 8 bits, 8 in 16) in a group of lanes.  Which token stands
+// in which row of S^T is free; they are dealt so that a lane's weights are the tokens kTok g ..
 // of its own group, which is what it loads of V.
-template <typename T, typename C, int DP> struct Loaded {
-    // keys of tile (u, w): elements as the fragments of q are laid out; values: 16 tokens of element 16 n + l
-    static constexpr int kPer = 16 / (int)sizeof(C); // elements of a load
-    static constexpr int KL = DP / (4 * kPer), VL = sizeof(C) == 1 ? 1 : 2;
-    u32x4 k[4][KL], v[DP / 16][VL];
-};
-
+// What bounds it is memory: K of the next step is asked for as soon as K of this one is used, V
+// likewise, so that a wavefront has 8 to 16 KiB under way at any time.
 template <typename T> __device__ __forceinline__ Frag<T> from_f8(uint32_t lo, uint32_t hi);
 template <> __device__ __forceinline__ bf16x8 from_f8<bf16_t>(uint32_t lo, uint32_t hi)
 {
@@ -284,35 +282,37 @@ __device__ __forceinline__ bool sees(int p, int c, int window, int sinks)
     return c <= p && (p - c < window || c < sinks);
 }
 
-// Steps of 64 tokens that rows at positions pa .. pb go over (see attention.hip).
+// Steps of `size` tokens that rows at positions pa .. pb go over (see attention.hip).
 struct Steps {
     int first, from, count;
     __device__ __forceinline__ int at(int k) const { return k < first ? k : from + k - first; }
 };
-__device__ __forceinline__ Steps steps_of(int pa, int pb, int len, int window, int sinks)
+__device__ __forceinline__ Steps steps_of(int pa, int pb, int len, int window, int sinks, int size)
 {
-    const int end = min(pb + 1, len), step = (int)kKeyStep;
+    const int end = min(pb + 1, len);
     Steps s{0, 0, 0};
     if (end <= 0)
         return s;
     const int lo = window > pa ? 0 : pa - window + 1;
-    s.first = (min(sinks, end) + step - 1) / step;
-    s.from = max(lo / step, s.first);
-    s.count = s.first + max(0, (end + step - 1) / step - s.from);
+    s.first = (min(sinks, end) + size - 1) / size;
+    s.from = max(lo / size, s.first);
+    s.count = s.first + max(0, (end + size - 1) / size - s.from);
     return s;
 }
 
+// A row and head's sums over some tokens, in a workspace of dim + 4 floats: maximum (base 2), sum of
+// weights, 2 unused, sums of values.
 template <typename T, typename C, int DP, int NC>
 __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
 {
     constexpr bool kF8 = sizeof(C) == 1;
     constexpr int NS = DP / 32, ND = DP / 16, COLS = 16 * NC;
-    typedef Loaded<T, C, DP> L;
+    constexpr int kTok = 16 / (int)sizeof(C), kStep = 4 * kTok, NT = kTok / 4, KL = DP / (4 * kTok);
     __shared__ float out[4][COLS][DP + 4]; // by wavefront; 4 more: no two columns on the same banks
     __shared__ float part_m[4][COLS], part_sum[4][COLS];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
-    const int dim = (int)a.c.dim, page = (int)a.c.page;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
+    const int dim = (int)a.c.dim, page = (int)a.c.page, shift = __builtin_ctz(a.c.page);
     const uint32_t group = a.heads / a.c.heads;
     uint32_t id = blockIdx.x;
     const uint32_t head = id % a.c.heads;
@@ -324,6 +324,11 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
     const int cols = (int)(s.n * group), m0 = (int)tile * COLS;
     if (m0 >= cols)
         return;
+    const int pa = s.first + m0 / (int)group, pb = s.first + (min(m0 + COLS, cols) - 1) / (int)group;
+    const Steps st = steps_of(pa, pb, a.c.npages ? s.len : 0, a.window, a.sinks, kStep);
+    // every share but the last has a.share steps
+    const int k0 = (int)min((uint64_t)split * a.share, (uint64_t)st.count);
+    const int k1 = split + 1 == a.splits ? st.count : min(k0 + (int)a.share, st.count);
 
     Frag<T> qf[NC][NS];
     int pos[NC];
@@ -338,16 +343,55 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
             qf[n][t] = m < cols && d < dim ? load_frag(qp + d) : zero_frag<T>();
         }
     }
-    const int pa = s.first + m0 / (int)group, pb = s.first + (min(m0 + COLS, cols) - 1) / (int)group;
-    const Steps st = steps_of(pa, pb, s.len, a.window, a.sinks);
-    const int each = (st.count + (int)a.splits - 1) / (int)a.splits;
-    const int k0 = (int)split * each, k1 = min(k0 + each, st.count);
     const uint32_t *const table = a.s.table + (uint64_t)b * a.s.table_stride;
     const float sc = a.scale * kLog2e;
 
+    // Pages of the tokens that a lane loads keys of, and values of, in step k; tokens that are not
+    // there are loaded from page 0 and hidden.
+    struct Pages {
+        uint32_t k, v;
+    };
+    auto pages_of = [&](int k) __attribute__((always_inline)) {
+        const int c0 = st.at(k) * kStep, ck = c0 + kTok * (l >> 2), cv = c0 + kTok * g;
+        return Pages{ck < s.len ? table[ck >> shift] : a.c.npages, cv < s.len ? table[cv >> shift] : a.c.npages};
+    };
+    u32x4 kr[NT][KL], vr[ND];
+    float k_scale = 1.0f, v_scale = 1.0f;
+    bool there = false; // the page of this lane's values
+    auto load_k = [&](int k, const Pages &p) __attribute__((always_inline)) {
+        const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
+        const int ck = st.at(k) * kStep + kTok * (l >> 2);
+        const C *const kp = (const C *)a.c.k + (((uint64_t)(p.k < a.c.npages ? p.k : 0) * a.c.heads + head) * page +
+                                                (ck & (page - 1)) + (l & 3)) * dim;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int t = 0; t < KL; ++t) // elements past the head's are met by zeros of q
+                kr[i][t] = *(const u32x4 *)(kp + 4 * i * dim + min(t * 4 * kTok + g * kTok, dim - kTok));
+    };
+    auto load_v = [&](int k, const Pages &p) __attribute__((always_inline)) {
+        const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
+        const int cv = st.at(k) * kStep + kTok * g;
+        const uint64_t unit = (uint64_t)(p.v < a.c.npages ? p.v : 0) * a.c.heads + head;
+        const C *const vp = (const C *)a.c.v + unit * page * dim + (cv & (page - 1));
+#pragma unroll
+        for (int d = 0; d < ND; ++d) // sums of elements past the head's are not stored
+            vr[d] = *(const u32x4 *)(vp + min(16 * d + l, dim - 1) * page);
+    };
+    auto load_scales = [&](const Pages &p) __attribute__((always_inline)) {
+        there = p.v < a.c.npages;
+        if constexpr (kF8) {
+            const uint64_t unit = (uint64_t)(there ? p.v : 0) * a.c.heads + head;
+            k_scale = a.c.k_scale[unit];
+            v_scale = a.c.v_scale[unit];
+        }
+    };
+
     f32x4 acc[ND][NC];
     float m[NC], sum[NC], ref;
-    for (int careful = 0; careful < 2; ++careful) { // see attend_kernel
+    // Values that are not finite reach rows that do not see them as 0 x inf: such a result is
+    // computed once more, carefully (see attend_kernel).
+    auto pass = [&](auto careful) __attribute__((always_inline)) {
         ref = 0.0f;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
@@ -357,65 +401,22 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
             for (int d = 0; d < ND; ++d)
                 acc[d][n] = f32x4{0, 0, 0, 0};
         }
-        for (int k = k0 + wave; k < k1; k += 4) {
-            const int c0 = st.at(k) * (int)kKeyStep;
-            // pages of the 16 tokens that this lane loads keys of, and values of
-            const int ck = c0 + 16 * (l >> 2), cg = c0 + 16 * g;
-            const uint32_t pk = ck < s.len ? table[ck / page] : a.c.npages;
-            const uint32_t pv = cg < s.len ? table[cg / page] : a.c.npages;
-            const bool in_k = pk < a.c.npages, in_v = pv < a.c.npages;
-            L x;
-            const C *const kp = (const C *)a.c.k + (((uint64_t)(in_k ? pk : 0) * a.c.heads + head) * page + ck % page + (l & 3)) * dim;
-            const C *const vp = (const C *)a.c.v + ((uint64_t)(in_v ? pv : 0) * a.c.heads + head) * page * dim + cg % page;
+        int k = k0 + wave;
+        if (k >= k1)
+            return false;
+        Pages next = pages_of(k);
+        load_k(k, next);
+        load_scales(next);
+        load_v(k, next);
+        auto step = [&](auto more) __attribute__((always_inline)) {
+            const int c0 = st.at(k) * kStep, c9 = c0 + kStep - 1, cg = c0 + kTok * g;
+            const bool in_v = there;
+            float ks = sc * k_scale, vs = v_scale;
+            if constexpr (more.value)
+                next = pages_of(k + 4);
+            f32x4 sv[NT][NC];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int t = 0; t < L::KL; ++t) {
-                    const int d = t * 4 * L::kPer + g * L::kPer;
-                    x.k[i][t] = u32x4{0, 0, 0, 0};
-                    if (in_k && d < dim)
-                        x.k[i][t] = *(const u32x4 *)(kp + 4 * i * dim + d);
-                }
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int t = 0; t < L::VL; ++t) {
-                    x.v[d][t] = u32x4{0, 0, 0, 0};
-                    if (in_v && 16 * d + l < dim)
-                        x.v[d][t] = *(const u32x4 *)(vp + (uint64_t)(16 * d + l) * page + t * L::kPer);
-                }
-            float ks = sc, vs = 1.0f;
-            if constexpr (kF8) {
-                const uint64_t at = (uint64_t)(in_v ? pv : 0) * a.c.heads + head;
-                ks = sc * a.c.k_scale[at];
-                vs = a.c.v_scale[at];
-            }
-            // Tokens that no row of the tile sees (not there yet, left of the window) may hold
-            // anything: their values become 0.  Edges only, all else is a whole step.
-            const int c9 = c0 + (int)kKeyStep - 1;
-            const bool whole = c9 <= pa && (pb - c0 < a.window || c9 < a.sinks) && __all(in_v);
-            if (!whole) {
-#pragma unroll
-                for (int t = 0; t < L::VL; ++t)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t mask = 0;
-#pragma unroll
-                        for (int e = 0; e < L::kPer / 4; ++e) {
-                            const int c = cg + t * L::kPer + w * (L::kPer / 4) + e;
-                            const bool seen = in_v && c <= pb && (c < a.sinks || pa - c < a.window);
-                            mask |= seen ? (kF8 ? 0xffu << 8 * e : 0xffffu << 16 * e) : 0;
-                        }
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-                            x.v[d][t][w] &= mask;
-                    }
-                if (!in_v || cg > pb || !(cg < a.sinks || pa - (cg + 15) < a.window))
-                    ks = vs = 0.0f; // a scale that belongs to nothing seen
-            }
-            f32x4 sv[4][NC];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < NT; ++i) {
 #pragma unroll
                 for (int n = 0; n < NC; ++n)
                     sv[i][n] = f32x4{0, 0, 0, 0};
@@ -423,56 +424,103 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
                 for (int t = 0; t < NS; ++t) {
                     Frag<T> f;
                     if constexpr (kF8)
-                        f = from_f8<T>(x.k[i][t / 2][2 * (t % 2)], x.k[i][t / 2][2 * (t % 2) + 1]);
+                        f = from_f8<T>(kr[i][t / 2][2 * (t % 2)], kr[i][t / 2][2 * (t % 2) + 1]);
                     else
-                        f = __builtin_bit_cast(Frag<T>, x.k[i][t]);
+                        f = __builtin_bit_cast(Frag<T>, kr[i][t]);
 #pragma unroll
                     for (int n = 0; n < NC; ++n)
                         sv[i][n] = mma(f, qf[n][t], sv[i][n]);
                 }
+                if constexpr (NC > 1 && DP > 64) // not every tile's keys widened at once
+                    __builtin_amdgcn_sched_barrier(0);
             }
-            // sv[i][n][j]: token cg + 4 i + j
+            if constexpr (more.value) {
+                load_k(k + 4, next);
+                load_scales(next);
+            }
+            // Tokens that no row of the tile sees (not there yet, left of the window) may hold
+            // anything: their values become 0.  Edges only, all else is a whole step.
+            const bool whole = c9 <= pa && (pb - c0 < a.window || c9 < a.sinks) && __all(in_v);
+            if (!whole) {
+                asm volatile(""); // a branch, not selects
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t mask = 0;
+#pragma unroll
+                    for (int e = 0; e < kTok / 4; ++e) {
+                        const int c = cg + w * (kTok / 4) + e;
+                        const bool seen = in_v && c <= pb && (c < a.sinks || pa - c < a.window);
+                        mask |= seen ? (kF8 ? 0xffu << 8 * e : 0xffffu << 16 * e) : 0;
+                    }
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        vr[d][w] &= mask;
+                }
+                if (!in_v || cg > pb || !(cg < a.sinks || pa - (cg + kTok - 1) < a.window))
+                    ks = vs = 0.0f; // a scale that belongs to nothing seen
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int n = 0; n < NC; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (in_v && sees(pos[n], cg + 4 * i + j, a.window, a.sinks))
+                                sv[i][n][j] *= ks;
+                            else
+                                sv[i][n][j] = kNegInf;
+                ks = 1.0f;
+            }
+            // acc is in units of the largest scale of values so far
             float to_ref = 1.0f, weigh = 1.0f;
-            if constexpr (kF8) { // acc is in units of the largest scale of values so far
+            if constexpr (kF8) {
                 const float top = fmaxf(ref, column_max(fabsf(vs)));
                 to_ref = top > 0 ? ref / top : 0.0f;
                 weigh = top > 0 ? vs / top : vs;
                 ref = top;
             }
+            float top[NC];
+            bool grown = kF8 && to_ref != 1.0f;
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-                float top = kNegInf;
+                top[n] = kNegInf;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < NT; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        float y = sv[i][n][j] * ks;
-                        if (!whole && !(in_v && sees(pos[n], cg + 4 * i + j, a.window, a.sinks)))
-                            y = kNegInf;
-                        sv[i][n][j] = y;
-                        top = fmaxf(top, y);
+                        sv[i][n][j] *= ks;
+                        top[n] = fmaxf(top[n], sv[i][n][j]);
                     }
-                top = fmaxf(m[n], column_max(top));
-                const float base = top == kNegInf ? 0.0f : top;
-                const float down = __builtin_amdgcn_exp2f(m[n] - base), less = base - WeightShift<T>::value;
-                m[n] = top;
+                top[n] = column_max(top[n]);
+                grown |= top[n] > m[n] + kSlack;
+            }
+            if (__any(grown)) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    const float to = fmaxf(m[n], top[n]);
+                    const float down = __builtin_amdgcn_exp2f(m[n] - (to == kNegInf ? 0.0f : to));
+                    m[n] = to;
+                    sum[n] *= down;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        acc[d][n] *= kF8 ? down * to_ref : down;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const float less = (m[n] == kNegInf ? 0.0f : m[n]) - WeightShift<T>::value;
                 float add = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < NT; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float p = __builtin_amdgcn_exp2f(sv[i][n][j] - less);
                         add += p;
                         sv[i][n][j] = kF8 ? p * weigh : p;
                     }
-                sum[n] = sum[n] * down + add;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    acc[d][n] *= kF8 ? down * to_ref : down;
+                sum[n] += add;
             }
-            const bool one_by_one = careful && !whole;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NT / 2; ++u) {
                 Frag<T> pf[NC];
 #pragma unroll
                 for (int n = 0; n < NC; ++n)
@@ -481,52 +529,57 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> f;
                     if constexpr (kF8)
-                        f = from_f8<T>(x.v[d][0][2 * u], x.v[d][0][2 * u + 1]);
+                        f = from_f8<T>(vr[d][2 * u], vr[d][2 * u + 1]);
                     else
-                        f = __builtin_bit_cast(Frag<T>, x.v[d][u]);
-                    if (one_by_one) {
+                        f = __builtin_bit_cast(Frag<T>, vr[d]);
+                    if constexpr (careful.value) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            if (!(fabsf((float)f[j]) < __builtin_inff()))
+                            if (!whole && !(fabsf((float)f[j]) < __builtin_inff()))
                                 f[j] = (T)0.0f;
                     }
 #pragma unroll
                     for (int n = 0; n < NC; ++n)
                         acc[d][n] = mma(f, pf[n], acc[d][n]);
+                    if constexpr (NC > 1 && DP > 64)
+                        if (d % 4 == 3)
+                            __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (one_by_one) {
-                for (int c = c0; c <= min(c9, pb); ++c) {
-                    const uint32_t pc = table[c / page];
-                    if (pc >= a.c.npages)
-                        continue;
-                    const C *const from = (const C *)a.c.v + ((uint64_t)pc * a.c.heads + head) * page * dim + c % page;
-                    for (int d = 0; d < ND; ++d)
-                        for (int j = 0; j < 4; ++j) {
-                            const int e = 16 * d + 4 * g + j;
-                            if (e >= dim)
-                                continue;
-                            float y;
-                            if constexpr (kF8)
-                                y = __builtin_amdgcn_cvt_pk_f32_fp8((int)from[(uint64_t)e * page], false)[0];
-                            else
-                                y = (float)from[(uint64_t)e * page];
-                            if (fabsf(y) < __builtin_inff())
-                                continue;
+            if constexpr (careful.value) {
+                if (!whole)
+                    for (int c = c0; c <= min(c9, pb); ++c) {
+                        const uint32_t pc = table[c >> shift];
+                        if (pc >= a.c.npages)
+                            continue;
+                        const C *const from = (const C *)a.c.v + ((uint64_t)pc * a.c.heads + head) * page * dim + (c & (page - 1));
 #pragma unroll
-                            for (int n = 0; n < NC; ++n)
-                                if (sees(pos[n], c, a.window, a.sinks)) {
+                        for (int d = 0; d < ND; ++d)
 #pragma unroll
-                                    for (int dd = 0; dd < ND; ++dd) // registers have no run-time number
+                            for (int j = 0; j < 4; ++j) {
+                                const int e = min(16 * d + 4 * g + j, dim - 1);
+                                asm volatile("" ::: "memory"); // one at a time: registers matter here, not time
+                                float y;
+                                if constexpr (kF8)
+                                    y = __builtin_amdgcn_cvt_pk_f32_fp8((int)from[e * page], false)[0];
+                                else
+                                    y = (float)from[e * page];
+                                if (fabsf(y) < __builtin_inff())
+                                    continue;
 #pragma unroll
-                                        for (int jj = 0; jj < 4; ++jj)
-                                            if (dd == d && jj == j)
-                                                acc[dd][n][jj] += y;
-                                }
-                        }
-                }
+                                for (int n = 0; n < NC; ++n)
+                                    if (sees(pos[n], c, a.window, a.sinks))
+                                        acc[d][n][j] += y;
+                            }
+                    }
             }
-        }
+            if constexpr (more.value)
+                load_v(k + 4, next);
+            k += 4;
+        };
+        while (k + 4 < k1)
+            step(std::true_type());
+        step(std::false_type());
         bool bad = false;
 #pragma unroll
         for (int n = 0; n < NC; ++n)
@@ -535,9 +588,10 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     bad |= pos[n] >= 0 && !(fabsf(acc[d][n][j]) < __builtin_inff());
-        if (careful || !__any(bad))
-            break;
-    }
+        return (bool)__any(bad);
+    };
+    if (pass(std::false_type()))
+        pass(std::true_type());
 
     // the four wavefronts joined, in their order
 #pragma unroll
@@ -574,7 +628,8 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
         const uint32_t h = head * group + mm % (int)group;
         if (a.splits > 1) {
             float *const to = a.partial + ((row * a.heads + h) * a.splits + split) * (dim + 4);
-            *(f32x4 *)(to + 4 + d) = y;
+            if (k0 < k1)
+                *(f32x4 *)(to + 4 + d) = y;
             if (d == 0) {
                 to[0] = top;
                 to[1] = total;
@@ -588,33 +643,62 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
     }
 }
 
-// The splits of a row and head joined, in their order; a wavefront for each, four elements a lane.
-template <typename T> __global__ __launch_bounds__(kThreads) void read_join_kernel(ReadArgs a)
+// The shares of a row and head joined: 32 lanes for its elements, WAYS such groups that take every
+// WAYS-th share and are then added in their order.
+template <typename T, int WAYS> __global__ __launch_bounds__(kThreads) void read_join_kernel(ReadArgs a)
 {
-    const uint32_t lane = threadIdx.x & 31, dim = a.c.dim;
-    const uint64_t at = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / 32;
-    if (at >= (uint64_t)a.s.rows * a.heads)
-        return;
-    const uint64_t row = at / a.heads;
+    constexpr int kRows = kThreads / (32 * WAYS);
+    __shared__ float sums[kRows][WAYS][32][5];
+    const uint32_t lane = threadIdx.x & 31, way = threadIdx.x / 32 % WAYS, mine = threadIdx.x / (32 * WAYS), dim = a.c.dim;
+    const uint64_t at = (uint64_t)blockIdx.x * kRows + mine, row = at / a.heads;
     const uint32_t h = (uint32_t)(at % a.heads);
-    const uint32_t b = seq_of_row(a.s, (uint32_t)row);
-    const Seq s = seq_of(a.s, b, a.c.page);
-    if (row < s.row0 || row - s.row0 >= s.n)
-        return;
+    bool there = at < (uint64_t)a.s.rows * a.heads;
+    if (there) {
+        const Seq s = seq_of(a.s, seq_of_row(a.s, (uint32_t)row), a.c.page);
+        there = row >= s.row0 && row - s.row0 < s.n;
+    }
     const float *const part = a.partial + at * a.splits * (dim + 4);
     float top = kNegInf;
-    for (uint32_t i = 0; i < a.splits; ++i)
-        top = fmaxf(top, part[i * (dim + 4)]);
+    if (there)
+        for (uint32_t i = lane; i < a.splits; i += 32)
+            top = fmaxf(top, part[i * (uint64_t)(dim + 4)]);
+#pragma unroll
+    for (int x = 16; x; x >>= 1)
+        top = fmaxf(top, __shfl_xor(top, x));
     const float base = top == kNegInf ? 0.0f : top;
     float total = 0.0f;
     f32x4 y = {0, 0, 0, 0};
-    for (uint32_t i = 0; i < a.splits; ++i) {
-        const float *const p = part + i * (dim + 4);
-        const float by = __builtin_amdgcn_exp2f(p[0] - base);
-        total += p[1] * by;
-        if (4 * lane < dim)
-            y += *(const f32x4 *)(p + 4 + 4 * lane) * by;
+    if (there) {
+#pragma unroll 4
+        for (uint32_t i = way; i < a.splits; i += WAYS) {
+            const float *const p = part + i * (uint64_t)(dim + 4);
+            if (p[0] == kNegInf)
+                continue; // nothing seen in this share, or no tokens: no sums either
+            const float by = __builtin_amdgcn_exp2f(p[0] - base);
+            total += p[1] * by;
+            if (4 * lane < dim)
+                y += *(const f32x4 *)(p + 4 + 4 * lane) * by;
+        }
     }
+    if constexpr (WAYS > 1) {
+        float *const to = sums[mine][way][lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            to[j] = y[j];
+        to[4] = total;
+        __syncthreads();
+        if (way)
+            return;
+#pragma unroll
+        for (int w = 1; w < WAYS; ++w) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[j] += sums[mine][w][lane][j];
+            total += sums[mine][w][lane][4];
+        }
+    }
+    if (!there)
+        return;
     const float by = total == 0.0f ? 0.0f : 1.0f / total;
     if (4 * lane < dim)
         store_half<T>((T *)a.o.p + row * a.o.stride + h * dim + 4 * lane, y * by);
@@ -629,10 +713,11 @@ template <typename T, typename C, int DP> hipError_t launch_read_one(const ReadA
         hipLaunchKernelGGL((read_kernel<T, C, DP, 1>), grid, block, 0, s, a);
     else
         hipLaunchKernelGGL((read_kernel<T, C, DP, 2>), grid, block, 0, s, a);
-    if (a.splits > 1) {
-        const uint64_t all = (uint64_t)a.s.rows * a.heads * 32;
-        hipLaunchKernelGGL((read_join_kernel<T>), dim3((uint32_t)((all + kThreads - 1) / kThreads)), block, 0, s, a);
-    }
+    const uint64_t rows = (uint64_t)a.s.rows * a.heads;
+    if (a.splits > 8)
+        hipLaunchKernelGGL((read_join_kernel<T, 8>), dim3((uint32_t)rows), block, 0, s, a);
+    else if (a.splits > 1)
+        hipLaunchKernelGGL((read_join_kernel<T, 1>), dim3((uint32_t)((rows + 7) / 8)), block, 0, s, a);
     return hipGetLastError();
 }
 
@@ -657,6 +742,7 @@ template <typename T> hipError_t launch_append(const AppendArgs &a, hipStream_t 
 } // namespace
 
 uint32_t read_columns(uint32_t max_rows, uint32_t group) { return (uint64_t)max_rows * group <= 16 ? 16 : 32; }
+uint32_t read_step(int cache_dtype) { return cache_dtype == 4 ? 64 : 32; }
 
 hipError_t launch_cache_append(const AppendArgs &a, hipStream_t stream)
 {
