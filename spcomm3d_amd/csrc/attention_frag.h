@@ -203,7 +203,7 @@ template <> struct WeightShift<f16_t> { static constexpr float value = 8.0f; };
 
 // The same number, of which the compiler knows nothing more: addresses made from it inside a loop
 // are made there again instead of being kept in registers that the accumulators need.
-__device__ __forceinline__ int fresh(int x)
+template <typename T> __device__ __forceinline__ T fresh(T x)
 {
     asm volatile("" : "+v"(x));
     return x;

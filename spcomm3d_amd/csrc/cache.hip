@@ -302,8 +302,9 @@ __device__ __forceinline__ Steps steps_of(int pa, int pb, int len, int window, i
 
 // A row and head's sums over some tokens, in a workspace of dim + 4 floats: maximum (base 2), sum of
 // weights, 2 unused, sums of values.
-template <typename T, typename C, int DP, int NC>
-__global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
+// ONE: a row for each sequence.  Its heads all see the same tokens.
+template <typename T, typename C, int DP, int NC, bool ONE>
+__global__ __launch_bounds__(kThreads, ONE && NC == 1 && (sizeof(C) == 2 || DP == 64) ? 3 : 2) void read_kernel(ReadArgs a)
 {
     constexpr bool kF8 = sizeof(C) == 1;
     constexpr int NS = DP / 32, ND = DP / 16, COLS = 16 * NC;
@@ -317,9 +318,10 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
     uint32_t id = blockIdx.x;
     const uint32_t head = id % a.c.heads;
     id /= a.c.heads;
-    const uint32_t split = id % a.splits;
-    id /= a.splits;
-    const uint32_t tile = id % a.col_tiles, b = id / a.col_tiles;
+    // first shares first: those that short sequences do not have come last, when slots are free
+    const uint32_t tile = id % a.col_tiles;
+    id /= a.col_tiles;
+    const uint32_t b = id % a.s.nseq, split = id / a.s.nseq;
     const Seq s = seq_of(a.s, b, a.c.page);
     const int cols = (int)(s.n * group), m0 = (int)tile * COLS;
     if (m0 >= cols)
@@ -329,6 +331,16 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
     // every share but the last has a.share steps
     const int k0 = (int)min((uint64_t)split * a.share, (uint64_t)st.count);
     const int k1 = split + 1 == a.splits ? st.count : min(k0 + (int)a.share, st.count);
+    if (k0 >= k1 && a.splits > 1) { // no tokens for this share
+        if (tid < COLS && m0 + tid < cols) {
+            const int mm = m0 + tid;
+            const uint64_t row = s.row0 + mm / (int)group;
+            float *const to = a.partial + ((row * a.heads + head * group + mm % (int)group) * a.splits + split) * (dim + 4);
+            to[0] = kNegInf;
+            to[1] = 0.0f;
+        }
+        return;
+    }
 
     Frag<T> qf[NC][NS];
     int pos[NC];
@@ -361,13 +373,15 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
     auto load_k = [&](int k, const Pages &p) __attribute__((always_inline)) {
         const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
         const int ck = st.at(k) * kStep + kTok * (l >> 2);
-        const C *const kp = (const C *)a.c.k + (((uint64_t)(p.k < a.c.npages ? p.k : 0) * a.c.heads + head) * page +
-                                                (ck & (page - 1)) + (l & 3)) * dim;
+        const C *kp = (const C *)a.c.k + (((uint64_t)(p.k < a.c.npages ? p.k : 0) * a.c.heads + head) * page +
+                                          (ck & (page - 1)) + (l & 3)) * dim;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < NT; ++i) {
 #pragma unroll
             for (int t = 0; t < KL; ++t) // elements past the head's are met by zeros of q
-                kr[i][t] = *(const u32x4 *)(kp + 4 * i * dim + min(t * 4 * kTok + g * kTok, dim - kTok));
+                kr[i][t] = *(const u32x4 *)(kp + min(t * 4 * kTok + g * kTok, dim - kTok));
+            kp = fresh(kp + 4 * dim); // one address, not all at once
+        }
     };
     auto load_v = [&](int k, const Pages &p) __attribute__((always_inline)) {
         const int lane = fresh(tid & 63), l = lane & 15, g = lane >> 4;
@@ -431,7 +445,7 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
                     for (int n = 0; n < NC; ++n)
                         sv[i][n] = mma(f, qf[n][t], sv[i][n]);
                 }
-                if constexpr (NC > 1 && DP > 64) // not every tile's keys widened at once
+                if constexpr (DP > 64 && (kF8 || NC > 1)) // not every tile's keys widened at once
                     __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (more.value) {
@@ -464,7 +478,7 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
                     for (int n = 0; n < NC; ++n)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (in_v && sees(pos[n], cg + 4 * i + j, a.window, a.sinks))
+                            if (in_v && sees(ONE ? pa : pos[n], cg + 4 * i + j, a.window, a.sinks))
                                 sv[i][n][j] *= ks;
                             else
                                 sv[i][n][j] = kNegInf;
@@ -541,8 +555,8 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
 #pragma unroll
                     for (int n = 0; n < NC; ++n)
                         acc[d][n] = mma(f, pf[n], acc[d][n]);
-                    if constexpr (NC > 1 && DP > 64)
-                        if (d % 4 == 3)
+                    if constexpr (DP > 64 && (kF8 || NC > 1))
+                        if (d % 2 == 1)
                             __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -581,6 +595,8 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
             step(std::true_type());
         step(std::false_type());
         bool bad = false;
+        if constexpr (ONE)
+            return bad; // no value is hidden from one and seen by another
 #pragma unroll
         for (int n = 0; n < NC; ++n)
 #pragma unroll
@@ -591,7 +607,8 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
         return (bool)__any(bad);
     };
     if (pass(std::false_type()))
-        pass(std::true_type());
+        if constexpr (!ONE)
+            pass(std::true_type());
 
     // the four wavefronts joined, in their order
 #pragma unroll
@@ -628,8 +645,7 @@ __global__ __launch_bounds__(kThreads, 2) void read_kernel(ReadArgs a)
         const uint32_t h = head * group + mm % (int)group;
         if (a.splits > 1) {
             float *const to = a.partial + ((row * a.heads + h) * a.splits + split) * (dim + 4);
-            if (k0 < k1)
-                *(f32x4 *)(to + 4 + d) = y;
+            *(f32x4 *)(to + 4 + d) = y;
             if (d == 0) {
                 to[0] = top;
                 to[1] = total;
@@ -709,10 +725,15 @@ template <typename T, int WAYS> __global__ __launch_bounds__(kThreads) void read
 template <typename T, typename C, int DP> hipError_t launch_read_one(const ReadArgs &a, hipStream_t s)
 {
     const dim3 grid(a.s.nseq * a.col_tiles * a.splits * a.c.heads), block(kThreads);
-    if (read_columns(a.s.max_rows, a.heads / a.c.heads) == 16)
-        hipLaunchKernelGGL((read_kernel<T, C, DP, 1>), grid, block, 0, s, a);
+    const bool narrow = read_columns(a.s.max_rows, a.heads / a.c.heads) == 16;
+    if (a.s.max_rows == 1 && narrow)
+        hipLaunchKernelGGL((read_kernel<T, C, DP, 1, true>), grid, block, 0, s, a);
+    else if (a.s.max_rows == 1)
+        hipLaunchKernelGGL((read_kernel<T, C, DP, 2, true>), grid, block, 0, s, a);
+    else if (narrow)
+        hipLaunchKernelGGL((read_kernel<T, C, DP, 1, false>), grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((read_kernel<T, C, DP, 2>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((read_kernel<T, C, DP, 2, false>), grid, block, 0, s, a);
     const uint64_t rows = (uint64_t)a.s.rows * a.heads;
     if (a.splits > 8)
         hipLaunchKernelGGL((read_join_kernel<T, 8>), dim3((uint32_t)rows), block, 0, s, a);
