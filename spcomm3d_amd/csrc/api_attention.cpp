@@ -802,13 +802,14 @@ int spc3d_cache_attend(spc3d_ctx *ctx, spc3d_cache *cache, const spc3d_cache_seq
     const uint64_t groups = (uint64_t)seqs->nseq * tiles * a.c.heads;
     // Shares of a sequence's steps: such that the longest sequences would make eight workgroups for each
     // CU (of sequences of several lengths most are shorter, and a share that has no tokens ends at
-    // once), but at least a step for each of a workgroup's four wavefronts.
+    // once), but at least a step for each of a workgroup's four wavefronts; none for few steps, which
+    // end sooner than a second launch would (700 tokens, 22 steps of 32: 7.6 us, in shares 10.0).
     const uint64_t step = read_step(a.c.dtype);
     uint64_t steps = ((uint64_t)seqs->max_len + step - 1) / step;
     if (a.window != INT_MAX)
         steps = std::min(steps, ((uint64_t)window + a.s.max_rows + step - 1) / step + 1 + ((uint64_t)a.sinks + step - 1) / step);
     const uint64_t share = groups * steps / (8ull * ctx->cu_count);
-    a.share = (uint32_t)std::max<uint64_t>(4, (share + 3) / 4 * 4);
+    a.share = (uint32_t)(steps <= 24 ? 24 : std::max<uint64_t>(4, (share + 3) / 4 * 4));
     a.splits = (uint32_t)std::max<uint64_t>(1, (steps + a.share - 1) / a.share);
     a.col_tiles = (uint32_t)tiles;
     if (groups * a.splits > INT_MAX || (uint64_t)seqs->rows * q->heads / 8 > INT_MAX)
