@@ -766,6 +766,10 @@ int spc3d_cache_append(spc3d_ctx *ctx, spc3d_cache *cache, const spc3d_cache_seq
         a.turned = rotations->n;
     }
     a.dtype = dt;
+    // A head of a page for each workgroup while there are few, four where that still leaves eight
+    // workgroups a CU: what they look up before they begin is then a smaller part.
+    a.each = pages / 4 >= 8ull * ctx->cu_count ? 4 : 1;
+    a.rows_each = seqs->rows / 4 >= 8ull * ctx->cu_count ? 4 : 1;
     HIP_TRY(launch_cache_append(a, ctx->stream));
     return SPC3D_OK;
 }

@@ -28,6 +28,8 @@ struct AppendArgs {
     HeadsView k, v, q, q_out; // q.p null: no queries to rotate
     const float *rotations;   // [position][turned]: cosines, then sines; null: none
     uint32_t turned, q_heads;
+    uint32_t each;      // heads of a page that a workgroup takes
+    uint32_t rows_each; // rows of queries: 1 or 4
     int dtype; // of the panels
 };
 

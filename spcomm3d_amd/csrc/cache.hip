@@ -26,10 +26,30 @@ __device__ __forceinline__ Seq seq_of(const SeqsView &s, uint32_t b, uint32_t pa
 }
 
 // ---- append -----------------------------------------------------------------------------------
-// Eight elements from d on of the row at `p`, rotated by the angles of position `pos`: pairs
-// (j, j + turned / 2).  Products and sums are rounded one by one, as the formula is written.
-template <typename T>
-__device__ __forceinline__ f32x8 rotated(const T *p, int d, const float *rotations, int turned, int64_t pos)
+// What rotates eight elements of a head, from d on: cosines and sines of their angles, and where the other
+// one of each pair (j, j + turned / 2) is.
+struct Turn {
+    f32x8 cos, sin;
+    int other; // element of the other; negative: nothing to rotate
+    float sign;
+};
+__device__ __forceinline__ Turn turn_of(const float *rotations, int turned, int64_t pos, int d)
+{
+    Turn t;
+    t.other = -1;
+    if (rotations && d < turned) {
+        const int half = turned / 2, at = d < half ? d : d - half;
+        const float *const c = rotations + pos * turned + at;
+        t.cos = load_frag(c);
+        t.sin = load_frag(c + half);
+        t.other = d < half ? d + half : at;
+        t.sign = d < half ? -1.0f : 1.0f;
+    }
+    return t;
+}
+// Eight elements from d on of the row at `p`, rotated.  Products and sums are rounded one by one, as the
+// formula is written.
+template <typename T> __device__ __forceinline__ f32x8 rotated(const T *p, int d, const Turn &t)
 {
 #pragma clang fp contract(off)
     const Frag<T> x = load_frag(p + d);
@@ -37,17 +57,18 @@ __device__ __forceinline__ f32x8 rotated(const T *p, int d, const float *rotatio
 #pragma unroll
     for (int j = 0; j < 8; ++j)
         y[j] = (float)x[j];
-    if (!rotations || d >= turned)
-        return y;
-    const int half = turned / 2, at = d < half ? d : d - half;
-    const Frag<T> z = load_frag(p + (d < half ? d + half : d - half));
-    const float *const c = rotations + pos * turned + at;
-    const f32x8 cos = load_frag(c), sin = load_frag(c + half);
-    const float sign = d < half ? -1.0f : 1.0f;
+    if (t.other >= 0) {
+        const Frag<T> z = load_frag(p + t.other);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        y[j] = y[j] * cos[j] + sign * ((float)z[j] * sin[j]);
+        for (int j = 0; j < 8; ++j)
+            y[j] = y[j] * t.cos[j] + t.sign * ((float)z[j] * t.sin[j]);
+    }
     return y;
+}
+template <typename T>
+__device__ __forceinline__ f32x8 rotated(const T *p, int d, const float *rotations, int turned, int64_t pos)
+{
+    return rotated(p, d, turn_of(rotations, turned, pos, d));
 }
 
 // The smallest 2^e, -40 <= e <= 40, with most <= 448 * 2^e.
@@ -84,7 +105,7 @@ __device__ __forceinline__ void unpack_f8(u32x2 w, float *x)
 // and the re-rounding of what it holds need no other's word.  C: what the cache holds.
 template <typename T, typename C>
 __device__ __forceinline__ void append_page(const AppendArgs &a, uint32_t b, uint32_t nth, uint32_t head, bool values,
-                                            float *reduce)
+                                            float *reduce, T *tile)
 {
     constexpr bool kF8 = sizeof(C) == 1;
     const Seq s = seq_of(a.s, b, a.c.page);
@@ -106,14 +127,22 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, uint32_t b, uin
     const float *const rot = values ? nullptr : a.rotations;
     // panel row of slot j: row0 + (p page + j - first)
     const int64_t row0 = (int64_t)s.row0 + (int64_t)p * page - s.first;
-    const int chunks = dim / 8;
+    const int chunks = dim / 8, wide = dim + 8;
 
+    // Values come by row and go by element, through LDS: 16 bytes a lane either way.
+    if (values && !kF8)
+        for (int i = tid; i < (hi - lo) * chunks; i += kThreads) {
+            const int j = lo + i / chunks, d = i % chunks * 8;
+            *(Frag<T> *)(tile + j * wide + d) = load_frag(src + (row0 + j) * from.stride + d);
+        }
     float scale = 1.0f, ratio = 1.0f;
     if constexpr (kF8) {
         float most = 0.0f;
         for (int i = tid; i < (hi - lo) * chunks; i += kThreads) {
             const int j = lo + i / chunks, d = i % chunks * 8;
             const f32x8 x = rotated(src + (row0 + j) * from.stride, d, rot, (int)a.turned, (int64_t)p * page + j);
+            if (values)
+                *(Frag<T> *)(tile + j * wide + d) = load_frag(src + (row0 + j) * from.stride + d);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (fabsf(x[e]) < __builtin_inff())
@@ -166,22 +195,33 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, uint32_t b, uin
         }
         return;
     }
-    // values: eight slots of one element at a time
+    if (!kF8)
+        __syncthreads(); // (8 bits: there was one since the tile was written)
+    // eight slots of one element at a time, the slots of an element next to each other
     const int first = from_slot / 8, blocks = (hi + 7) / 8 - first;
     for (int i = tid; i < blocks * dim; i += kThreads) {
-        const int d = i % dim, j0 = (first + i / dim) * 8;
+        const int d = i / blocks, j0 = (first + i - d * blocks) * 8;
         C *const to = dst + (uint64_t)d * page + j0;
+        const bool all = j0 >= lo && j0 + 8 <= hi; // nothing of what was there stays
         T x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            x[e] = j0 + e >= lo && j0 + e < hi ? src[(row0 + j0 + e) * (int64_t)from.stride + d] : (T)0.0f;
+            x[e] = all || (j0 + e >= lo && j0 + e < hi) ? tile[(j0 + e) * wide + d] : (T)0.0f;
         if constexpr (kF8) {
-            float y[8], old[8];
-            const u32x2 was = *(const u32x2 *)to;
-            unpack_f8(was, old);
+            float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                y[e] = j0 + e < lo ? old[e] * ratio : (float)x[e] / scale;
+                y[e] = (float)x[e] / scale;
+            u32x2 was = {0, 0};
+            if (!all) {
+                float old[8];
+                was = *(const u32x2 *)to;
+                unpack_f8(was, old);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (j0 + e < lo)
+                        y[e] = old[e] * ratio;
+            }
             u32x2 w = pack_f8(y);
             if (j0 + 8 > hi) { // slots that no token has yet keep what they hold
                 const int keep = hi - j0;
@@ -194,10 +234,12 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, uint32_t b, uin
             }
             *(u32x2 *)to = w;
         } else {
-            Frag<C> f = *(const Frag<C> *)to;
+            Frag<C> f = zero_frag<C>();
+            if (!all)
+                f = *(const Frag<C> *)to;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (j0 + e >= lo && j0 + e < hi)
+                if (all || (j0 + e >= lo && j0 + e < hi))
                     f[e] = (C)x[e];
             *(Frag<C> *)to = f;
         }
@@ -218,35 +260,63 @@ __device__ __forceinline__ uint32_t seq_of_row(const SeqsView &s, uint32_t row)
     return lo;
 }
 
-template <typename T, typename C> __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, uint32_t per_seq)
+// A row of queries, rotated by `lanes` of which this is number `lane`: one keeps its place in a head from one load to the next where heads
+// divide them, and its angles with it.
+template <typename T> __device__ __forceinline__ void turn_queries(const AppendArgs &a, uint32_t row, int lane, int lanes)
 {
-    __shared__ float reduce[kThreads / 64];
-    const uint32_t pages = a.s.nseq * per_seq * a.c.heads * 2;
-    uint32_t id = blockIdx.x;
-    if (id < pages) {
-        const bool values = id & 1;
-        id >>= 1;
-        const uint32_t head = id % a.c.heads;
-        id /= a.c.heads;
-        append_page<T, C>(a, id / per_seq, id % per_seq, head, values, reduce);
-        return;
-    }
-    const uint32_t row = id - pages; // a row of queries
     const uint32_t b = seq_of_row(a.s, row);
     const Seq s = seq_of(a.s, b, a.c.page);
     if (row < s.row0 || row - s.row0 >= s.n)
         return;
-    const int pos = s.first + (int)(row - s.row0), dim = (int)a.c.dim, chunks = dim / 8;
+    const int pos = s.first + (int)(row - s.row0), dim = (int)a.c.dim, chunks = dim / 8, all = (int)a.q_heads * chunks;
+    const float *const rotations = pos < 0 ? nullptr : a.rotations;
     const T *const src = (const T *)a.q.p + row * a.q.stride;
     T *const dst = (T *)a.q_out.p + row * a.q_out.stride;
-    for (int i = threadIdx.x; i < (int)a.q_heads * chunks; i += kThreads) {
-        const int h = i / chunks, d = i % chunks * 8;
-        const f32x8 y = rotated(src + h * dim, d, pos < 0 ? nullptr : a.rotations, (int)a.turned, pos);
+    const int ahead = lanes / chunks, more = lanes % chunks; // heads and chunks from one load to the next
+    int h = lane / chunks, c = lane % chunks;
+    Turn t = turn_of(rotations, (int)a.turned, pos, c * 8);
+#pragma unroll 4
+    for (int i = lane; i < all; i += lanes) {
+        if (more)
+            t = turn_of(rotations, (int)a.turned, pos, c * 8);
+        const f32x8 y = rotated(src + h * dim, c * 8, t);
         Frag<T> f;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             f[e] = (T)y[e];
-        *(Frag<T> *)(dst + h * dim + d) = f;
+        *(Frag<T> *)(dst + h * dim + c * 8) = f;
+        h += ahead;
+        c += more;
+        if (c >= chunks) {
+            c -= chunks;
+            ++h;
+        }
+    }
+}
+
+// Workgroups: first those of pages, a.each heads of a page's keys or values each, then those of queries, a.rows_each
+// rows each.
+template <typename T, typename C> __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, uint32_t per_seq)
+{
+    __shared__ float reduce[kThreads / 64];
+    extern __shared__ __align__(16) char tile[]; // page rows of dim + 8 elements
+    const uint32_t parts = (a.c.heads + a.each - 1) / a.each, pages = a.s.nseq * per_seq * parts * 2;
+    uint32_t id = blockIdx.x;
+    if (id >= pages) {
+        const uint32_t lanes = kThreads / a.rows_each;
+        const uint32_t row = (id - pages) * a.rows_each + __builtin_amdgcn_readfirstlane(threadIdx.x / lanes);
+        if (row < a.s.rows)
+            turn_queries<T>(a, row, (int)(threadIdx.x % lanes), (int)lanes);
+        return;
+    }
+    const bool values = id & 1;
+    id >>= 1;
+    const uint32_t first = id % parts * a.each, end = min(first + a.each, a.c.heads);
+    id /= parts;
+    for (uint32_t head = first; head < end; ++head) {
+        if (head > first)
+            __syncthreads(); // the last head's maxima and values are read
+        append_page<T, C>(a, id / per_seq, id % per_seq, head, values, reduce, (T *)tile);
     }
 }
 
@@ -752,11 +822,12 @@ template <typename T> hipError_t launch_read(const ReadArgs &a, hipStream_t s)
 template <typename T> hipError_t launch_append(const AppendArgs &a, hipStream_t s)
 {
     const uint32_t per_seq = (a.s.max_rows + a.c.page - 2) / a.c.page + 1; // pages that so many rows touch
-    const uint64_t grid = (uint64_t)a.s.nseq * per_seq * a.c.heads * 2 + (a.q.p ? a.s.rows : 0);
+    const uint32_t parts = (a.c.heads + a.each - 1) / a.each, lds = a.c.page * (a.c.dim + 8) * sizeof(T);
+    const uint64_t grid = (uint64_t)a.s.nseq * per_seq * parts * 2 + (a.q.p ? (a.s.rows + a.rows_each - 1) / a.rows_each : 0);
     if (a.c.dtype == 4)
-        hipLaunchKernelGGL((append_kernel<T, uint8_t>), dim3((uint32_t)grid), dim3(kThreads), 0, s, a, per_seq);
+        hipLaunchKernelGGL((append_kernel<T, uint8_t>), dim3((uint32_t)grid), dim3(kThreads), lds, s, a, per_seq);
     else
-        hipLaunchKernelGGL((append_kernel<T, T>), dim3((uint32_t)grid), dim3(kThreads), 0, s, a, per_seq);
+        hipLaunchKernelGGL((append_kernel<T, T>), dim3((uint32_t)grid), dim3(kThreads), lds, s, a, per_seq);
     return hipGetLastError();
 }
 
