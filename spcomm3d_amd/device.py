@@ -16,7 +16,20 @@ _NP = {capi.F32: np.dtype(np.float32), capi.F64: np.dtype(np.float64)}
 # Types of panels beside those of SDDMM and SpMM, by name; bfloat16 and e4m3 have no numpy type
 # and are uploaded and downloaded as their bits.
 _SHORT = {"bf16": (capi.BF16, np.dtype(np.uint16)), "f16": (capi.F16, np.dtype(np.float16)),
-          "f8": (capi.F8, np.dtype(np.uint8))}
+          "e4m3": (capi.F8, np.dtype(np.uint8))}  # ("f8" is numpy's name for float64)
+_CACHED = {"bf16": capi.BF16, "f16": capi.F16, "f8": capi.F8, "e4m3": capi.F8}
+
+
+def to_bf16(x) -> np.ndarray:
+    """The bits of ``x`` in bfloat16, rounded to nearest even: what a ``"bf16"`` panel is uploaded from."""
+    b = np.ascontiguousarray(x, dtype=np.float32).view(np.uint32)
+    r = ((b + 0x7FFF + ((b >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where((b & 0x7FFFFFFF) > 0x7F800000, np.uint16(0x7FC0), r)
+
+
+def from_bf16(bits) -> np.ndarray:
+    """The float32 numbers of a downloaded ``"bf16"`` panel."""
+    return (np.asarray(bits, dtype=np.uint16).astype(np.uint32) << 16).view(np.float32)
 
 
 def dtype_code(dtype) -> int:
@@ -367,7 +380,7 @@ class Cache:
         (``spc3d_cache_wrap``) instead of allocating."""
         self.ctx, self.dtype = ctx, dtype
         self.pages, self.page, self.heads, self.dim = int(pages), int(page), int(heads), int(dim)
-        code = _SHORT[dtype][0] if dtype in _SHORT else dtype_code(dtype)
+        code = _CACHED[dtype] if dtype in _CACHED else dtype_code(dtype)
         h = ctypes.c_void_p()
         if k is None and v is None:
             check(ctx._lib.spc3d_cache_create(ctx._h, code, self.pages, self.page, self.heads, self.dim,

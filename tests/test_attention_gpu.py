@@ -302,7 +302,7 @@ def test_refusals(ctx):
 
     P = s.panels
     f32 = ctx.panel(22, 256, "f32")
-    f8 = ctx.panel(22, 256, "f8")
+    f8 = ctx.panel(22, 256, "e4m3")
     odd = ctx.panel(22, 260, "bf16")
     short = ctx.panel(19, 256, "bf16")
     small = ctx.vals(79, np.float32)
@@ -360,7 +360,7 @@ def test_refusals(ctx):
     s.close()
 
 
-@pytest.mark.parametrize("dtype,one", [("bf16", 0x3F80), ("f16", np.float16(1.0)), ("f8", 0x38)])
+@pytest.mark.parametrize("dtype,one", [("bf16", 0x3F80), ("f16", np.float16(1.0)), ("e4m3", 0x38)])
 def test_panels_of_the_short_types(ctx, dtype, one):
     p, q = ctx.panel(5, 7, dtype), ctx.panel(5, 7, dtype)
     p.fill(1.0)

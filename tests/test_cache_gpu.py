@@ -456,3 +456,14 @@ def test_refusals(ctx):
     for x in (f32, half.panel, short.panel, rot, few, wide, odd, small, inside):
         x.close()
     w.close()
+
+
+def test_example_from_training_to_serving(ctx):
+    """The example's own two parts.  An 8-bit value is off by 1/16 of itself at most and half the
+    largest scale's spacing; keys move scores by as much of their size, so that a few tenths of an
+    output's size is the most that a token may be off."""
+    from spcomm3d_amd import attention_example as example
+
+    losses = example.fit(ctx, steps=30)
+    assert losses[-1] < 0.8 * losses[0] and all(b < a for a, b in zip(losses, losses[1:]))
+    assert example.serve(ctx) < 0.3
