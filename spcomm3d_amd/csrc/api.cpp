@@ -4,6 +4,7 @@
 // host memory in api_host_calls.cpp.  No CPU compute fallback: without a device every
 // device call fails.
 #include "api_internal.h"
+#include "attention.h"
 
 // ---- partial-sum rows for the SpMM entry point that allocates nothing ---------------
 // spc3d_spmm_noalloc keeps the partial sums of cut rows here instead of in memory the
@@ -493,7 +494,9 @@ int spc3d_panel_fill(spc3d_panel *p, double value)
     int rc = use_device(p->ctx, true);
     if (rc)
         return rc;
-    HIP_TRY(launch_fill(p->dtype, p->dev, (uint64_t)p->m * p->n, value, p->ctx->stream));
+    const uint64_t n = (uint64_t)p->m * p->n;
+    HIP_TRY(dtype_ok(p->dtype) ? launch_fill(p->dtype, p->dev, n, value, p->ctx->stream)
+                               : launch_fill_short(p->dtype, p->dev, n, (float)value, p->ctx->stream));
     return SPC3D_OK;
 }
 

@@ -73,6 +73,8 @@ struct BandArgs {
 hipError_t launch_attend(const BandArgs &a, uint32_t tile_rows, hipStream_t stream);
 hipError_t launch_attend_dq(const BandArgs &a, uint32_t tile_rows, hipStream_t stream);
 hipError_t launch_attend_dkv(const BandArgs &a, hipStream_t stream);
+// Panels of the types that only these calls take.
+hipError_t launch_fill_short(int dtype, void *p, uint64_t n, float value, hipStream_t stream);
 uint64_t partial_floats(uint32_t nslots, uint32_t kv_heads, uint32_t dim);
 
 } // namespace spc3d

@@ -5,7 +5,6 @@
 //   dQ_i = scale sum_c dS_ic k_c,  dK_c = scale sum_i dS_ic q_i.
 #include "attention.h"
 #include "attention_frag.h"
-#include "kernels.h"
 
 #include <type_traits>
 
@@ -774,6 +773,8 @@ hipError_t launch_attend_dkv(const BandArgs &a, hipStream_t stream)
 
 hipError_t launch_fill_short(int dtype, void *p, uint64_t n, float value, hipStream_t stream)
 {
+    if (n == 0)
+        return hipSuccess;
     const uint32_t grid = (uint32_t)((n + kThreads - 1) / kThreads < 4096 ? (n + kThreads - 1) / kThreads : 4096);
     hipLaunchKernelGGL(fill_short_kernel, dim3(grid), dim3(kThreads), 0, stream, dtype, p, n, value);
     return hipGetLastError();

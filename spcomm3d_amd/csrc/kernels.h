@@ -171,8 +171,6 @@ hipError_t launch_probe_cols(uint32_t *col, uint64_t n, uint32_t mode, uint32_t 
 // dst[0..bytes) = src[0..bytes); both 16-byte aligned, non-overlapping
 hipError_t launch_copy(void *dst, const void *src, uint64_t bytes, hipStream_t stream);
 hipError_t launch_fill(int dtype, void *p, uint64_t n, double value, hipStream_t stream);
-// The same for the types of the attention calls (attention.hip).
-hipError_t launch_fill_short(int dtype, void *p, uint64_t n, float value, hipStream_t stream);
 
 // Name of the kernel variant launch_sddmm / launch_spmm picks for (dtype, K);
 // for logs and profiles.

@@ -3232,8 +3232,6 @@ hipError_t launch_fill(int dtype, void *p, uint64_t n, double value, hipStream_t
 {
     if (n == 0)
         return hipSuccess;
-    if (dtype > 1)
-        return launch_fill_short(dtype, p, n, (float)value, stream);
     if (dtype == 1)
         hipLaunchKernelGGL((fill_kernel<double>), dim3(stream_grid(n)), dim3(kBlock), 0, stream,
                            (double *)p, n, value);
