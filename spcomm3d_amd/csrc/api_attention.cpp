@@ -382,8 +382,11 @@ BandArgs args_of(const spc3d_band *b, const spc3d_heads *q, const spc3d_heads *k
     a.scale = scale;
     a.dtype = q->panel->dtype;
     // Tiles of 128 rows read K and V half as often; of 64 rows there are twice as many.  The large
-    // ones are taken from two for each CU on.
-    const int i = (uint64_t)b->ntiles[1] * q->heads >= 2ull * b->ctx->cu_count;
+    // ones are taken from two for each CU on, for small heads from 11 / 4 on (causal, 64 / 128 rows, us;
+    // heads of 128: 256 tiles 89 / 107, 512 70 / 69, 640 92 / 79, 1024 213 / 170; heads of 64: 512
+    // 38 / 45, 640 51 / 56, 704 66 / 62, 800 80 / 71).
+    const uint64_t large = (uint64_t)b->ntiles[1] * q->heads;
+    const int i = 4 * large >= (q->dim > 64 ? 8ull : 11ull) * b->ctx->cu_count;
     *tile_rows = i ? 128 : 64;
     a.tiles = b->tiles[i];
     a.ntiles = b->ntiles[i];

@@ -65,6 +65,9 @@ template <typename T> __device__ __forceinline__ bool is_finite(T x) { return fa
 // Each wavefront owns 16 NQ rows; K and V come through LDS in steps of 64 columns.  S^T = K Q^T
 // leaves lane l with row l % 16, so maxima and sums of a row are over the lane's own registers and
 // two exchanges, and the probabilities are the right operand of O^T += V^T P^T where they lie.
+// Bound by the matrix units and, between their instructions, by the exponentials: 16,384 rows in bfloat16,
+// 32 heads of 128 over 8, window 4096: 1.05 ms, 0.92 PFLOP/s (8192^3 product of the library: 1.23).
+// Short or few rows are bound by the launch and the chain of steps: 48 rows, 4 heads of 64: 4.4 us.
 template <typename T, int DP, int NQ>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kernel(BandArgs a)
 {
@@ -284,7 +287,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_kerne
 // ---- backward -------------------------------------------------------------------------------
 // Two kernels, one over rows (dQ) and one over columns (dK, dV), each with the scores computed
 // again: seven products instead of five, but every sum is one workgroup's, in a fixed order,
-// without atomics or a panel of partial dQ.
+// without atomics or a panel of partial dQ.  Bound by the matrix units, the exponentials and the reads of
+// LDS between them.  8192 rows in bfloat16, 32 heads of 128 over 8, window 1024: dQ 277 us, dK and dV
+// 455, forward 217 before them.
 template <typename T, int DP, int NQ>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dq_kernel(BandArgs a)
 {
@@ -678,7 +683,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
         }
 }
 
-// The pieces of a tile of columns joined in their order.
+// The pieces of a tile of columns joined in their order.  Bound by the chain of loads of one element's
+// pieces: 6 us for the sinks of 8192 rows, 11 to 13 us where every tile is cut.
 template <typename T> __global__ __launch_bounds__(kThreads) void join_dkv_kernel(BandArgs a)
 {
     const KeySplit t = a.splits[blockIdx.x];
