@@ -127,7 +127,7 @@ uint64_t makespan(const std::vector<uint64_t> &costs, size_t slots)
 
 // Tiles of kKeyTile columns, each with the rows that see one of them, cut into pieces of steps
 // where that ends sooner.  Rows that see a tile for its sinks alone are pieces of their own.
-// The choice goes by what the parts of a call cost on an MI355X, in steps (64 rows, 7 us with
+// The choice goes by what the parts of a call cost on an MI355X, in steps (64 rows, 6 us with
 // two workgroups on a CU, heads of 128 in 16 bits): half a step to begin and end a piece, two more
 // to write its partial sums, half a step of the whole GPU for the launch that joins them and 1/512
 // for each piece in it.
