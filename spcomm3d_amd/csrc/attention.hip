@@ -685,7 +685,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attend_dkv_k
 
 // The pieces of a tile of columns joined in their order.  Bound by the chain of loads of one element's
 // pieces, so four elements a lane and four pieces at a time: 5 us for the sinks of 8192 rows, 5 and 10 us where
-// every tile is cut (1000 rows in single precision; 7700 in bfloat16), where one element and piece took 6, 13 and 12.
+// every tile is cut (1000 rows in single precision; 6000 in bfloat16), where one element and piece took 6, 13 and 12.
 template <typename T> __global__ __launch_bounds__(kThreads) void join_dkv_kernel(BandArgs a)
 {
     const KeySplit t = a.splits[blockIdx.x];
