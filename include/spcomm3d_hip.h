@@ -596,7 +596,9 @@ SPC3D_API int spc3d_attend(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *
  *     dQ_i = scale sum_c dS_ic k_c,   dK_c = scale sum_i dS_ic q_i,   dV_c = sum_i P_ic dO_i,
  * the last two over every head that shares the column's.  Overwrites dq, dk, dv (columns that no
  * row sees get 0); runs give the same bits.  The outputs overlap neither the inputs nor each
- * other.  Asynchronous on the context's stream, as spc3d_attend. */
+ * other.  The inputs are finite: spc3d_attend keeps what is not from rows that do not see it, here
+ * it may reach others of the same sequence.
+ * Asynchronous on the context's stream, as spc3d_attend. */
 SPC3D_API int spc3d_attend_grad(spc3d_ctx *ctx, spc3d_band *band, const spc3d_heads *q,
                       const spc3d_heads *k, const spc3d_heads *v, float scale,
                       const spc3d_heads *o, const spc3d_vals *lse, const spc3d_heads *d_o,
